@@ -401,7 +401,7 @@ def _own_pass(s):
                                    offsets=s["offsets"], rotary=s["plan"], q=s["q"])
         return {"q": q, "k": s["k"], "v": s["v"], "k_scale": s["k_scale"], "v_scale": s["v_scale"]}
     return {"out": pkg.attend_paged_cache(s["cache"], s["q"], s["page_table"], s["lengths"], offsets=s["offsets"],
-                                          max_new=s["max_new"], max_length=s["max_length"],
+                                          max_length=s["max_length"],
                                           window=c["window"] or None)}
 
 
