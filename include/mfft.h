@@ -320,6 +320,117 @@ int mfft_twiddle_transpose(const void* in, void* out, int64_t rows, int64_t cols
  * once (bench.py divides its per-size rates by it). */
 int mfft_stream_copy(const void* in, void* out, int64_t bytes, void* stream);
 
+/* ---- Language-model operators -------------------------------------------
+ * No counterpart in the reference.  Rotary positions multiply pairs of a
+ * head's channels, as complex values, by unit roots; a paged cache holds keys
+ * and values in 8 bits; attention reads it.  All calls enqueue on `stream`,
+ * allocate nothing and never synchronise the host; index arrays (positions,
+ * page tables, lengths) are device memory and are bounds-checked by the
+ * kernels: an entry out of range gives NaN (or is skipped, for the append) and
+ * never an access outside the caller's buffers. */
+
+/* element types of the tensors */
+enum { MFFT_F32 = 0, MFFT_F16 = 1, MFFT_BF16 = 2 };
+/* which channels of a head form pair j of r / 2: (j, j + r/2) or (2j, 2j + 1) */
+enum { MFFT_ROTARY_HALF = 0, MFFT_ROTARY_INTERLEAVED = 1 };
+
+typedef struct mfft_rotary mfft_rotary;
+
+/* Roots amplitude * exp(i p frequencies[j]) for positions p < max_positions
+ * (1..2^24) and j < pairs (1..256), on the current device: two tables, made
+ * in long double, of 1024 and ceil(max_positions / 1024) rows. */
+int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pairs, int64_t max_positions,
+                       double amplitude, int layout);
+/* As mfft_plan_destroy: frees the tables, does not synchronise. */
+int mfft_rotary_destroy(mfft_rotary* rotary);
+
+typedef struct {
+    const void* in;           /* [batch][tokens][heads][head_dim], strides in elements, channels adjacent */
+    void* out;                /* same shape; may be `in` itself with the same strides */
+    const void* positions;    /* [batch][tokens] int32 or int64 */
+    int64_t in_strides[3], out_strides[3], position_strides[2];
+    int64_t batch, tokens;
+    int32_t heads, head_dim;  /* head_dim >= 2 * pairs; the channels after them are copied */
+    int32_t dtype;            /* MFFT_F32 / F16 / BF16, of `in` and `out`; computed in 32 bits */
+    int32_t positions_64;     /* positions are int64 */
+    int32_t direction;        /* MFFT_FORWARD, or MFFT_INVERSE: the conjugate roots (the gradient) */
+} mfft_rotary_args;
+int mfft_rotary_execute(const mfft_rotary* rotary, const mfft_rotary_args* args, void* stream);
+
+/* A paged cache.  Codes are e4m3 (1 sign, 4 exponent, 3 fraction bits, bias 7,
+ * largest 448, one NaN, no infinities); a page's value is code * scale, the
+ * scale a power of two, the least one with every magnitude at most 448 * scale.
+ *   k        [pages][kv_heads][page_size][head_dim]
+ *   v        [pages][kv_heads][page_size / 16][head_dim][16]: sixteen tokens
+ *            of one channel side by side, what one lane of a matrix
+ *            instruction contracts over
+ *   k_scale, v_scale  [pages][kv_heads]
+ * head_dim 64, 96, 128 or 256; page_size a multiple of 16 up to 1024; codes
+ * 16-byte aligned. */
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t pages;
+    int32_t kv_heads, head_dim, page_size;
+} mfft_cache;
+
+/* Token i of sequence b goes to position starts[b] + i of that sequence: slot
+ * position mod page_size of page page_table[b][position / page_size].  With a
+ * rotary, k (and q, into q_out) is rotated by that position first, in 32 bits.
+ * Slot 0 opens a page anew; a page whose later tokens need a larger scale has
+ * its earlier codes rescaled (exactly, except for codes that fall below
+ * 2^-6 * scale).  Infinities and NaN are stored as NaN and do not count for
+ * the scale.  A page belongs to one sequence.  Positions past the table's
+ * width, and page numbers outside [0, pages), are skipped. */
+typedef struct {
+    const void* k;             /* [tokens][kv_heads][head_dim] */
+    const void* v;
+    const void* q;             /* NULL, or [tokens][q_heads][head_dim] */
+    void* q_out;
+    int64_t k_strides[2], v_strides[2], q_strides[2], q_out_strides[2];  /* token, head; in elements */
+    const int32_t* page_table; /* [sequences][table_width] */
+    const int32_t* starts;     /* [sequences]: tokens cached before this call */
+    const int32_t* offsets;    /* [sequences + 1]: sequence b's tokens are rows offsets[b] .. offsets[b + 1];
+                                  NULL: one token each */
+    int64_t table_stride, tokens;
+    int32_t table_width, sequences;
+    int32_t q_heads, dtype;
+} mfft_append_args;
+int mfft_cache_append(const mfft_cache* cache, const mfft_rotary* rotary, const mfft_append_args* args, void* stream);
+
+/* Attention of q [tokens][q_heads][head_dim] over the cache: q_heads a
+ * multiple of kv_heads, query head h reads key head h / (q_heads / kv_heads).
+ * Sequence b's n = offsets[b + 1] - offsets[b] queries are its last positions,
+ * lengths[b] - n + i; with `causal` each sees the keys up to its own
+ * position, with window > 0 only the last `window` of those positions (without
+ * `causal`: every key after position - window).  out = softmax(scale q k) v,
+ * 0 for a query that sees no key; lse (or NULL) its log of the sum of
+ * exponentials, -infinity there.  Scores, maxima and sums are 32-bit; the
+ * weights are rounded to the queries' type for the product with v. */
+typedef struct {
+    const void* q;
+    void* out;                 /* [tokens][q_heads][head_dim] */
+    float* lse;                /* [tokens][q_heads] or NULL */
+    int64_t q_strides[2], out_strides[2];
+    const int32_t* page_table;
+    const int32_t* lengths;    /* [sequences] */
+    const int32_t* offsets;    /* [sequences + 1], or NULL: tokens / sequences queries each */
+    int64_t table_stride, tokens;
+    int32_t table_width, sequences;
+    int32_t q_heads, dtype;    /* MFFT_F16 or MFFT_BF16 */
+    float scale;
+    int32_t causal;
+    int64_t window;            /* 0: none */
+    int64_t max_length;        /* 0, or a length the sequences are known not to exceed (longer ones still work) */
+    void* workspace;
+    int64_t workspace_bytes;
+} mfft_attend_args;
+/* Bytes of workspace (256-byte aligned) the call needs; from the shapes only. */
+int mfft_cache_attend_workspace(const mfft_cache* cache, const mfft_attend_args* args, int64_t* bytes);
+int mfft_cache_attend(const mfft_cache* cache, const mfft_attend_args* args, void* stream);
+
 /* Device facts for the profile / environment fingerprint. */
 int mfft_device_props_get(int device, mfft_device_props* out);
 

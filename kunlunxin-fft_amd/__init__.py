@@ -10,6 +10,11 @@ The package directory is ``kunlunxin-fft_amd``; it is imported under the
 module name ``kunlunxin_fft_amd`` (``__graft_entry__.load_package()`` or
 ``importlib`` with ``submodule_search_locations``).
 
+Beside the transforms stand the operators a language model's step needs next
+to them: rotary positions (``plan_rotary``, ``execute_rotary_plan``) and a
+paged 8-bit key and value cache with its attention (``PagedCache``,
+``append_paged_cache``, ``attend_paged_cache``).
+
 Host-only names (planning, tables, configs) import without torch;
 torch-dependent names (runners) resolve lazily on first access, as in the
 reference's ``src/xpu/__init__.py:37-81``.
@@ -42,6 +47,7 @@ from .entry import (  # noqa: F401
 )
 from .composition import composition_select, load_composition_table  # noqa: F401
 from .error_metric import max_rel_error, rel_l2  # noqa: F401
+from .rotary import RotaryPlan, RotaryScaling, execute_rotary_plan, plan_rotary  # noqa: F401
 from .selector import Selection, assert_current_environment, load_table, select  # noqa: F401
 
 _TORCH_ATTRS = {
@@ -68,6 +74,9 @@ _TORCH_ATTRS = {
     "fft_dit_matrix_packet_batch": "runner",
     "fft_dit_grouped": "runner",
     "fft_dif_grouped": "runner",
+    "PagedCache": "paged_cache",
+    "append_paged_cache": "paged_cache",
+    "attend_paged_cache": "paged_cache",
     "log2_exact": "validate",
     "time_call": "runner",
     "time_call_detailed": "runner",
@@ -79,10 +88,10 @@ _TORCH_ATTRS = {
 
 __all__ = [
     "ConfigError", "DesignSpace", "DeviceProfile", "ExecutionPlan",
-    "ExecutionReport", "Manifest", "Selection", "SizeMatrix", "SUPPORTED_NORMS", "SUPPORTED_TRANSFORMS",
+    "ExecutionReport", "Manifest", "RotaryPlan", "RotaryScaling", "Selection", "SizeMatrix", "SUPPORTED_NORMS", "SUPPORTED_TRANSFORMS",
     "SUPPORTED_TRANSFORM_DIRECTIONS", "assert_current_environment", "build_manifest",
-    "composition_select", "execute_fft_plan", "git_commit", "git_dirty",
-    "load_composition_table", "load_table", "max_rel_error", "norm_scale", "plan_fft", "rel_l2",
+    "composition_select", "execute_fft_plan", "execute_rotary_plan", "git_commit", "git_dirty",
+    "load_composition_table", "load_table", "max_rel_error", "norm_scale", "plan_fft", "plan_rotary", "rel_l2",
     "run_fft", "select",
     *sorted(_TORCH_ATTRS),
 ]

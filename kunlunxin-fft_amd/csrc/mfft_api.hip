@@ -30,8 +30,10 @@ thread_local LaunchTimer* g_timer = nullptr;
 static __device__ __align__(256) unsigned char scratch[MFFT_NOALLOC_SCRATCH_BYTES];
 
 namespace {
-
 thread_local std::string g_err;
+}
+
+namespace mfft {
 
 int fail(int code, const char* fmt, ...) {
     char buf[1024];
@@ -46,6 +48,15 @@ int fail(int code, const char* fmt, ...) {
 int hip_fail(hipError_t e, const char* what) {
     return fail(MFFT_ERR_RUNTIME, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
 }
+
+void clear_error() { g_err.clear(); }
+
+}  // namespace mfft
+
+namespace {
+
+using mfft::fail;
+using mfft::hip_fail;
 
 int log2_exact(int64_t n) {
     if (n <= 0 || (n & (n - 1)) != 0) return -1;
@@ -121,6 +132,10 @@ constexpr int kMaxDevices = 64;
 std::mutex g_upload_mu;
 hipStream_t g_upload[kMaxDevices] = {};
 
+}  // namespace
+
+namespace mfft {
+
 int upload_stream(int dev, hipStream_t* out) {
     if (dev < 0 || dev >= kMaxDevices) return fail(MFFT_ERR_RUNTIME, "device %d beyond %d devices", dev, kMaxDevices);
     std::lock_guard<std::mutex> lk(g_upload_mu);
@@ -148,6 +163,13 @@ int upload(float2** dptr, const std::vector<float2>& h, int64_t* bytes, hipStrea
     *bytes += (int64_t)nb;
     return MFFT_OK;
 }
+
+}  // namespace mfft
+
+namespace {
+
+using mfft::upload;
+using mfft::upload_stream;
 
 void release(mfft_plan* p) {
     float2** bufs[] = {&p->tw,      &p->tw_n1, &p->tw_n2, &p->tw_col, &p->tw_real,

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <vector>
+
 #include "../../include/mfft.h"
 
 struct mfft_plan {
@@ -56,6 +58,16 @@ struct mfft_plan {
 };
 
 namespace mfft {
+
+// ---- mfft_api.hip: what every C entry shares -------------------------------
+// Set the calling thread's message and return `code` / MFFT_ERR_RUNTIME.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int hip_fail(hipError_t e, const char* what);
+void clear_error();
+// The device's private upload stream, and an asynchronous upload of a host
+// table on it (the caller waits for the stream; `h` must live until then).
+int upload_stream(int dev, hipStream_t* out);
+int upload(float2** dptr, const std::vector<float2>& h, int64_t* bytes, hipStream_t us);
 
 // Optional per-launch event recording (mfft_execute_timed): every launcher
 // calls mark(stream) right after each kernel launch.  Off (nullptr) otherwise.
@@ -159,4 +171,35 @@ hipError_t launch_fourstep(int dir, const float2* src, float2* dst, char* fws, c
 hipError_t launch_fourstep_real(const float2* src, float2* dst, float2* work, const mfft_plan* p, float scale,
                                 hipStream_t stream);
 
+// ---- rotary_kernels.hip, append_kernels.hip, attend_kernels.hip ------------
+// Roots m exp(i p theta_j) of a position p are the product of a row of `lo`
+// (p mod 1024) and one of `hi` (p / 1024): see mfft_rotary below.
+constexpr int kRotaryLoLog2 = 10;
+struct RotaryTables {
+    const float2* lo;       // [1024][pairs]
+    const float2* hi;       // [ceil(max_positions / 1024)][pairs], the amplitude in it
+    int64_t max_positions;  // 0: no rotation
+    int32_t pairs;
+    int32_t layout;
+};
+hipError_t launch_rotary(const RotaryTables& t, const mfft_rotary_args& a, hipStream_t stream);
+bool rotary_launch_fits(const RotaryTables& t, const mfft_rotary_args& a);
+hipError_t launch_append(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, hipStream_t stream);
+bool append_launch_fits(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a);
+bool attend_supported(int head_dim);
+int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a);
+hipError_t launch_attend(const mfft_cache& c, const mfft_attend_args& a, hipStream_t stream);
+
 }  // namespace mfft
+
+// Two factors of the roots instead of one table of every position: 2^20
+// positions of 64 pairs take 1 MiB in place of 512 MiB, so a call's rows stay
+// in L2.  Both factors are made in long double and rounded once, as the
+// transforms' twiddles are; their product is within 2 ulp of the root.
+struct mfft_rotary {
+    int device = 0;
+    mfft::RotaryTables t{};
+    float2* lo = nullptr;
+    float2* hi = nullptr;
+    int64_t table_bytes = 0;
+};

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -41,8 +42,20 @@ EXPORTS = (
     "mfft_abi_version", "mfft_plan_sync_overruns", "mfft_plan_create_ex", "mfft_plan_workspace_size",
     "mfft_execute_ws", "mfft_execute_noalloc", "mfft_twiddle_transpose", "mfft_stream_copy",
     "mfft_r2c_stitch", "mfft_c2r_pre", "mfft_c2r_unpack",
+    "mfft_rotary_create", "mfft_rotary_destroy", "mfft_rotary_execute",
+    "mfft_cache_append", "mfft_cache_attend_workspace", "mfft_cache_attend",
 )
 PLAN_CALLER_WORKSPACE = 1
+
+# enums and argument structs of the language-model operators.  The structs
+# go to C as packed bytes: one pack is about a microsecond, filling a
+# ctypes.Structure field by field several.
+F32, F16, BF16 = 0, 1, 2
+LAYOUT_IDS = {"half": 0, "interleaved": 1}
+ROTARY_ARGS = struct.Struct("@3P10q5i4x")
+CACHE_ARGS = struct.Struct("@4Pq3i4x")
+APPEND_ARGS = struct.Struct("@4P8q3P2q4i")
+ATTEND_ARGS = struct.Struct("@3P4q3P2q4ifi2qPq")
 
 
 class PlanInfo(ctypes.Structure):
@@ -129,6 +142,19 @@ def load() -> ctypes.CDLL:
         lib.mfft_stream_copy.restype = i32
         lib.mfft_device_props_get.argtypes = [i32, ctypes.POINTER(DeviceProps)]
         lib.mfft_device_props_get.restype = i32
+        lib.mfft_rotary_create.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_double), ctypes.c_int32, i64,
+                                           ctypes.c_double, i32]
+        lib.mfft_rotary_create.restype = i32
+        lib.mfft_rotary_destroy.argtypes = [vp]
+        lib.mfft_rotary_destroy.restype = i32
+        lib.mfft_rotary_execute.argtypes = [vp, ctypes.c_char_p, vp]
+        lib.mfft_rotary_execute.restype = i32
+        lib.mfft_cache_append.argtypes = [ctypes.c_char_p, vp, ctypes.c_char_p, vp]
+        lib.mfft_cache_append.restype = i32
+        lib.mfft_cache_attend_workspace.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(i64)]
+        lib.mfft_cache_attend_workspace.restype = i32
+        lib.mfft_cache_attend.argtypes = [ctypes.c_char_p, ctypes.c_char_p, vp]
+        lib.mfft_cache_attend.restype = i32
         lib.mfft_last_error.argtypes = []
         lib.mfft_last_error.restype = ctypes.c_char_p
         lib.mfft_abi_version.argtypes = []
@@ -271,6 +297,46 @@ def release_retired(sync=None) -> int:
     for h, _ in items:
         _lib.mfft_plan_destroy(h)
     return len(items)
+
+
+class NativeRotary:
+    """Owner of one ``mfft_rotary*`` on the device current at creation.  Its
+    tables are at most a few MB and live as long as the process: the plans
+    that use it are memoised, and freeing it would need every stream done."""
+
+    __slots__ = ("handle", "device")
+
+    def __init__(self, frequencies, max_positions: int, amplitude: float, layout: str, device: int):
+        lib = load()
+        h = ctypes.c_void_p()
+        check(lib.mfft_rotary_create(ctypes.byref(h), (ctypes.c_double * len(frequencies))(*frequencies),
+                                     len(frequencies), int(max_positions), float(amplitude), LAYOUT_IDS[layout]))
+        self.handle = h
+        self.device = device
+
+
+def rotary_execute(rotary: NativeRotary, args: bytes, stream_ptr: int) -> None:
+    rc = _lib.mfft_rotary_execute(rotary.handle, args, stream_ptr)
+    if rc:
+        check(rc)
+
+
+def cache_append(cache: bytes, rotary: NativeRotary | None, args: bytes, stream_ptr: int) -> None:
+    rc = load().mfft_cache_append(cache, rotary.handle if rotary is not None else None, args, stream_ptr)
+    if rc:
+        check(rc)
+
+
+def cache_attend_workspace(cache: bytes, args: bytes) -> int:
+    k = ctypes.c_int64(0)
+    check(load().mfft_cache_attend_workspace(cache, args, ctypes.byref(k)))
+    return k.value
+
+
+def cache_attend(cache: bytes, args: bytes, stream_ptr: int) -> None:
+    rc = load().mfft_cache_attend(cache, args, stream_ptr)
+    if rc:
+        check(rc)
 
 
 def r2c_stitch(z_ptr: int, x_ptr: int, n: int, batch: int, scale: float, stream_ptr: int) -> None:
