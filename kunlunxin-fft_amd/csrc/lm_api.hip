@@ -271,6 +271,8 @@ static int check_attend(const mfft_cache* c, const mfft_attend_args* a) {
         return fail(MFFT_ERR_VALUE, "q_heads must be a multiple of the cache's %d heads, at most 65536, got %d", c->kv_heads, a->q_heads);
     if (!std::isfinite(a->scale) || a->scale < 0.0f) return fail(MFFT_ERR_VALUE, "scale must be finite and not negative");
     if (a->window < 0 || a->window > 0x7fffffff) return fail(MFFT_ERR_VALUE, "window must be in [0, 2^31)");
+    if ((int64_t)a->table_width * c->page_size > (int64_t)1 << 30)
+        return fail(MFFT_ERR_VALUE, "page_table holds more than 2^30 positions a sequence");
     if (a->max_length < 0) return fail(MFFT_ERR_VALUE, "max_length must not be negative");
     if (int rc = check_strides("q", {a->tokens, (int64_t)a->q_heads}, a->q_strides)) return rc;
     if (int rc = check_strides("out", {a->tokens, (int64_t)a->q_heads}, a->out_strides)) return rc;
@@ -300,6 +302,8 @@ int mfft_cache_attend(const mfft_cache* c, const mfft_attend_args* a, void* stre
     const Extent o = extent(a->out, {a->tokens, (int64_t)a->q_heads}, a->out_strides, D, 2);
     if (overlap(extent(a->q, {a->tokens, (int64_t)a->q_heads}, a->q_strides, D, 2), o))
         return fail(MFFT_ERR_VALUE, "q and out must not overlap");
+    if (!mfft::attend_launch_fits(*c, *a))
+        return fail(MFFT_ERR_UNSUPPORTED, "%lld tokens need a launch of 2^32 work-items or more; split the call", (long long)a->tokens);
     const int64_t need = mfft::attend_workspace(*c, *a);
     if (need > 0) {
         if (!a->workspace || a->workspace_bytes < need)

@@ -187,6 +187,7 @@ bool rotary_launch_fits(const RotaryTables& t, const mfft_rotary_args& a);
 hipError_t launch_append(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, hipStream_t stream);
 bool append_launch_fits(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a);
 bool attend_supported(int head_dim);
+bool attend_launch_fits(const mfft_cache& c, const mfft_attend_args& a);
 int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a);
 hipError_t launch_attend(const mfft_cache& c, const mfft_attend_args& a, hipStream_t stream);
 
