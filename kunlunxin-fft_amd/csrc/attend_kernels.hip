@@ -27,6 +27,7 @@ namespace mfft {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -44,6 +45,9 @@ struct Mat<__bf16> {
     static __device__ __forceinline__ f32x4 mfma(x8 a, x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
     template <bool HI>
     static __device__ __forceinline__ x2 decode(uint32_t w, float scale) {
         return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
@@ -55,6 +59,9 @@ struct Mat<_Float16> {
     typedef f16x2 x2;
     static __device__ __forceinline__ f32x4 mfma(x8 a, x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
     template <bool HI>
     static __device__ __forceinline__ x2 decode(uint32_t w, float scale) {
@@ -100,6 +107,17 @@ __device__ __forceinline__ u32x4 keep_bytes(int from, int to) {
     return r;
 }
 
+// the larger of v in lanes l and l ^ 32 (l ^ 16): the swaps exchange the upper
+// half (odd rows of sixteen) of one register with the lower (even) of another
+__device__ __forceinline__ float max_across_32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_across_16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // 0x01 in each byte that is a NaN code
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (((w & 0x7f7f7f7f) + 0x01010101) >> 7) & 0x01010101; }
 
@@ -118,16 +136,35 @@ __device__ __forceinline__ float log_sum(float m, float l, bool poison) {
 // lengths, which only the device knows; every workgroup works its place out for
 // itself with one pass of a wave over the sequences.  Cut items leave their
 // (m, l, O) in the workspace and join_kernel adds them up.
+// x / d of 0 <= x < 2^31, exact: with l the least so that d <= 2^l and
+// m = ceil(2^(31 + l) / d), floor(x m / 2^(31 + l)).  (A division by a number
+// that is no constant is about twenty instructions, and a 64-bit one a hundred
+// and fifty; code that runs once a launch is mostly time to fetch it.)
+struct Divisor {
+    uint32_t m, shift;
+};
+inline Divisor divisor(uint32_t d) {
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < d) ++l;
+    return {(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), 31 + l};
+}
+__device__ __forceinline__ int operator/(int x, Divisor d) { return (int)((uint64_t)(uint32_t)x * d.m >> d.shift); }
+
 struct AttendShape {
     int group;        // query heads a key head
-    int rows;         // rows of a block
+    Divisor by_group, by_heads;
+    int rows, log_rows;  // rows of a block, a power of two
     int units;        // page_size / 16
     uint64_t magic;   // floor(2^32 / units) + 1: x / units = x * magic >> 32, exact for x < 2^26
     int grid;         // shares; 0: one workgroup an item, none cut
     int least;        // fewest groups of 64 keys in a share
     int live;         // rows of a block that can be in use
+    int join_rows;    // rows of a workgroup of the join
     int64_t per;      // queries of each sequence without offsets
 };
+
+constexpr int kCUs = 256;
+constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
 
 // the item that starts in share i and is cut at its end: its parts are in
 // slots 2 i + 1, 2 (i + 1), 2 (i + 2), ... of the workspace
@@ -137,7 +174,7 @@ struct Cut {
 };
 
 struct Sequence {
-    int64_t row0, n;  // its queries
+    int row0, n;      // its queries
     int len;          // its keys, within the table
     bool poison;      // it has more than the table's
     int low, tiles;   // first key that any query sees (a multiple of 64), groups of 64 keys from there
@@ -146,8 +183,8 @@ struct Sequence {
 
 __device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_attend_args& a, const AttendShape& sh, int b) {
     Sequence q;
-    q.row0 = seq_offset(a.offsets, sh.per, a.tokens, b);
-    q.n = seq_offset(a.offsets, sh.per, a.tokens, b + 1) - q.row0;
+    q.row0 = (int)seq_offset(a.offsets, sh.per, a.tokens, b);
+    q.n = (int)seq_offset(a.offsets, sh.per, a.tokens, b + 1) - q.row0;
     if (q.n < 0) q.n = 0;
     const int most = a.table_width * c.page_size;
     const int len = a.lengths[b];
@@ -155,12 +192,12 @@ __device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_att
     q.len = len < 0 ? 0 : q.poison ? most : len;
     q.low = 0;
     if (a.window) {
-        const int64_t lo = q.len - q.n + 1 - a.window;
-        q.low = lo > 0 ? (int)(lo & ~(int64_t)63) : 0;
+        const int lo = q.len - q.n + 1 - (int)a.window;
+        q.low = lo > 0 ? lo & ~63 : 0;
     }
     q.tiles = (q.len - q.low + 63) >> 6;
     if (q.tiles < 1) q.tiles = 1;  // rows that see nothing are still written
-    q.blocks = (int)((q.n * sh.group + sh.rows - 1) / sh.rows);
+    q.blocks = (q.n * sh.group + sh.rows - 1) >> sh.log_rows;
     return q;
 }
 
@@ -179,47 +216,157 @@ __device__ __forceinline__ int here(int v) {
     return v;
 }
 
+// v is loaded by here.  A loop that uses v, loaded before it, otherwise waits in
+// every round for all loads, those for its next round among them: the waits are
+// placed for the first round.
+template <class V>
+__device__ __forceinline__ void loaded(V& v) {
+    asm volatile("" : "+v"(v));
+}
+
+// floor(x / d) of 0 <= x < 2^52, d > 0, the same in all lanes: a double's
+// quotient is off by one at most
+__device__ __forceinline__ int64_t quotient(int64_t x, int d) {
+    int64_t q = (int64_t)((double)x / (double)d);
+    if (q * d > x) --q;
+    if ((q + 1) * d <= x) ++q;
+    return uniform(q);
+}
+
+// sum over the wave up to and including this lane, without LDS: within sixteen
+// lanes by row shifts, then the rows before by broadcasts of their last lane
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int64_t o = __shfl_up(v, s);
-        if (lane >= s) v += o;
-    }
+    auto step = [&](auto ctrl, auto rows) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+        v += (int64_t)((uint64_t)hi << 32 | lo);
+    };
+    step(ic<0x111>{}, ic<0xf>{});  // row_shr 1, 2, 4, 8
+    step(ic<0x112>{}, ic<0xf>{});
+    step(ic<0x114>{}, ic<0xf>{});
+    step(ic<0x118>{}, ic<0xf>{});
+    step(ic<0x142>{}, ic<0xa>{});  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+    step(ic<0x143>{}, ic<0xc>{});
     return v;
 }
+__device__ __forceinline__ int64_t from_lane(int64_t v, int l) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)v, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
 
-// The sequence in whose work (groups of keys, or items where `by_item`) place
-// `at` lies, and what comes before it; -1 past the end.
-__device__ __forceinline__ int locate(const mfft_cache& c, const mfft_attend_args& a, const AttendShape& sh, bool by_item,
-                                      int64_t at, int64_t& before) {
-    const int lane = threadIdx.x & 63;
-    before = 0;
-    for (int i = 0; i < a.sequences; i += 64) {
-        int64_t w = 0;
-        if (i + lane < a.sequences) {
-            const Sequence q = sequence(c, a, sh, i + lane);
+// The list of all work: groups of keys (or items, where `by_item`), sequence
+// after sequence, 64 sequences at a time.
+struct WorkList {
+    const mfft_cache& c;
+    const mfft_attend_args& a;
+    const AttendShape& sh;
+    bool by_item;
+    int64_t w, upto;  // of the 64 sequences at hand: this lane's, and with those before
+
+    __device__ __forceinline__ void take(int i) {
+        const int b = i + (int)(threadIdx.x & 63);
+        w = 0;
+        if (b < a.sequences) {
+            const Sequence q = sequence(c, a, sh, b);
             w = (int64_t)q.blocks * c.kv_heads * (by_item ? 1 : q.tiles);
         }
-        const int64_t upto = wave_scan(w);
-        const uint64_t hit = __ballot(before + upto > at);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            before += uniform(__shfl(upto - w, l));
-            return uniform(i + l);
-        }
-        before += uniform(__shfl(upto, 63));
+        upto = wave_scan(w);
     }
-    return -1;
-}
-
-__device__ __forceinline__ int64_t all_work(const mfft_cache& c, const mfft_attend_args& a, const AttendShape& sh) {
-    int64_t none;
-    (void)locate(c, a, sh, false, INT64_MAX, none);
-    return none;
-}
+    __device__ __forceinline__ int64_t total() {
+        int64_t t = 0;
+        for (int i = 0; i < a.sequences; i += 64) {
+            take(i);
+            t += from_lane(upto, 63);
+        }
+        return t;
+    }
+    // the sequence in whose work place `at` lies, and what comes before it;
+    // -1 past the end.  `taken`: the first 64 sequences are at hand.
+    __device__ __forceinline__ int find(int64_t at, int64_t& before, bool taken) {
+        before = 0;
+        for (int i = 0; i < a.sequences; i += 64) {
+            if (!taken) take(i);
+            taken = false;
+            const uint64_t hit = __ballot(before + upto > at);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                before += from_lane(upto, l) - from_lane(w, l);
+                return uniform(i + l);
+            }
+            before += from_lane(upto, 63);
+        }
+        return -1;
+    }
+};
 
 // ---- one item, some of its keys --------------------------------------------------
+// What every form of the kernel needs of its item: pages and bounds.
+template <int D>
+struct Item {
+    const mfft_cache& c;
+    const mfft_attend_args& a;
+    const AttendShape& sh;
+    Sequence seq;
+    const int32_t* table;
+    int h;
+    int all, block;  // rows of the sequence and key head, first row of the block
+    int block_lo, block_hi, block_all_lo, block_all_hi;  // keys that any, and that all, rows of the block see
+
+    __device__ __forceinline__ Item(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_) : c(c_), a(a_), sh(sh_) {}
+
+    // the keys [lower, upper) that query `tok` of the sequence sees
+    __device__ __forceinline__ int lower(int tok) const { return a.window ? max(seq.len - seq.n + tok + 1 - (int)a.window, 0) : 0; }
+    __device__ __forceinline__ int upper(int tok) const {
+        return a.causal ? max(min(seq.len - seq.n + tok + 1, seq.len), 0) : seq.len;
+    }
+    __device__ __forceinline__ void take(int b, int block_, int h_, int rows) {
+        h = h_;
+        table = a.page_table + b * a.table_stride;
+        all = seq.n * sh.group;
+        block = block_ * rows;
+        nan_left = false;
+        // both ends of what a row sees rise with it
+        const int t0 = block / sh.by_group, t1 = (min(block + rows, all) - 1) / sh.by_group;
+        block_lo = lower(t0);
+        block_hi = upper(t1);
+        block_all_lo = lower(t1);
+        block_all_hi = upper(t0);
+    }
+
+    // Table entry of the sixteen keys `u` of the sequence, and where in the page
+    // they are.  Past the sequence's end the entry is its last page's (the
+    // table's first if it has none), so that loads need no branch: a branch
+    // around a load ends in a wait for all loads before it.
+    __device__ __forceinline__ int page_entry(uint32_t u) const {
+        const uint32_t most = seq.len > 0 ? (uint32_t)(seq.len - 1) >> 4 : 0;
+        return table[(uint32_t)(min(u, most) * sh.magic >> 32)];
+    }
+    __device__ __forceinline__ uint32_t unit_in_page(uint32_t u) const { return u - (uint32_t)(u * sh.magic >> 32) * sh.units; }
+    __device__ __forceinline__ int64_t page_of(int entry) const { return (uint32_t)entry < (uint32_t)c.pages ? entry : 0; }
+    // first byte of sixteen tokens' codes (keys: their first row; values: their unit)
+    __device__ __forceinline__ int64_t unit_at(int entry, uint32_t u) const {
+        return ((page_of(entry) * c.kv_heads + h) * sh.units + unit_in_page(u)) * (16 * D);
+    }
+    // Values of a group where not every row sees every key.  Keys that no row
+    // sees may hold anything: their codes count as 0 (`keep` masks the others).
+    // A NaN of the others counts only for the rows that see its key, while 0 * NaN
+    // is NaN: its code becomes 0 here, and mark_nans() finds the rows that see
+    // it once the item is done.
+    bool nan_left;
+    __device__ __forceinline__ u32x4 clean(u32x4 w, u32x4 keep) {
+        uint32_t bad = 0;
+        static_for<0, 4>([&](auto x) {
+            const uint32_t v = w[x.value] & keep[x.value], n = nan_bytes(v);
+            bad |= n;
+            w[x.value] = v & ~(n * 0xffu);
+        });
+        nan_left |= bad != 0;
+        return w;
+    }
+
+    __device__ __forceinline__ bool block_edge(int key0) const { return key0 < block_all_lo || key0 + 64 > block_all_hi; }
+};
+
 // KEYS: the workgroup's four waves share 16 R rows and take every fourth group
 // of 64 keys, each straight from memory into registers, one group ahead; their
 // (m, l, O) are joined in LDS.  For few rows: nothing but the cache's bytes
@@ -227,7 +374,7 @@ __device__ __forceinline__ int64_t all_work(const mfft_cache& c, const mfft_atte
 // not KEYS: each wave has 16 R rows of its own and all take every group, which
 // goes through LDS once for the four.  For many rows.
 template <class E, int D, int R, bool KEYS>
-struct Attend {
+struct Attend : Item<D> {
     using M = Mat<E>;
     typedef typename M::x8 x8;
     using S = Dims<D>;
@@ -250,17 +397,12 @@ struct Attend {
     };
     typedef typename std::conditional<KEYS, decltype(Shared::join), decltype(Shared::tile)>::type Lds;
 
-    const mfft_cache& c;
-    const mfft_attend_args& a;
-    const AttendShape& sh;
+    using I = Item<D>;
+    using I::a, I::c, I::sh, I::seq, I::h, I::all, I::block, I::nan_left;
     Lds& lds;
     int lane, wave, j, g, kg, kr;
 
     // of the item
-    Sequence seq;
-    const int32_t* table;
-    int h;
-    int64_t all, block;
     x8 qv[R][S::KK];
     int low[R], top[R];                // keys [low, top) that each of this lane's rows sees
     int all_lo, all_hi, any_lo, any_hi;  // and all, and any, of the wave's rows
@@ -274,7 +416,7 @@ struct Attend {
     float cs, vs;
 
     __device__ __forceinline__ Attend(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
-        : c(c_), a(a_), sh(sh_), lds(lds_) {
+        : I(c_, a_, sh_), lds(lds_) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         j = lane & 15;
@@ -283,34 +425,26 @@ struct Attend {
         kr = j & 3;
     }
 
-    __device__ __forceinline__ int64_t row_of(int r, int j) const { return block + (KEYS ? 0 : 16 * R * wave) + 16 * r + j; }
+    __device__ __forceinline__ int row_of(int r, int j) const { return block + (KEYS ? 0 : 16 * R * wave) + 16 * r + j; }
 
     __device__ __forceinline__ void begin(int b, int block_, int h_) {
-        h = h_;
-        table = a.page_table + b * a.table_stride;
-        all = seq.n * sh.group;
-        block = (int64_t)block_ * ROWS;
+        this->take(b, block_, h_, ROWS);
         all_lo = 0;
         all_hi = seq.len;
         any_lo = seq.len;
         any_hi = 0;
-        nan_left = false;
         const int j = here(this->j), g = here(this->g);
         static_for<0, R>([&](auto r) {
-            int64_t row = row_of(r.value, j);
-            row = row < all ? row : all - 1;  // rows past the last repeat it and are not stored
-            const int64_t tok = row / sh.group;
-            const int qh = h * sh.group + (int)(row % sh.group);
+            const int row = min(row_of(r.value, j), all - 1);  // rows past the last repeat it and are not stored
+            const int tok = row / sh.by_group;
+            const int qh = h * sh.group + row - tok * sh.group;
             const E* q = (const E*)a.q + (seq.row0 + tok) * a.q_strides[0] + qh * a.q_strides[1];
             static_for<0, S::J>([&](auto jj) {
                 qv[r.value][2 * jj.value] = *(const x8*)(q + 64 * jj.value + 16 * g);
                 qv[r.value][2 * jj.value + 1] = *(const x8*)(q + 64 * jj.value + 16 * g + 8);
             });
             if constexpr (S::REM) qv[r.value][S::KK - 1] = *(const x8*)(q + 64 * S::J + 8 * g);
-            const int64_t pos = seq.len - seq.n + tok;
-            int hi = a.causal && pos + 1 < seq.len ? (int)(pos + 1) : seq.len;
-            int lo = a.window && pos + 1 > a.window ? (int)(pos + 1 - a.window) : 0;
-            if (hi < lo) hi = lo;
+            const int lo = this->lower(tok), hi = max(this->upper(tok), lo);
             low[r.value] = lo;
             top[r.value] = hi;
             all_lo = max(all_lo, lo);
@@ -321,6 +455,7 @@ struct Attend {
             m[r.value] = kLowest;
             l[r.value] = 0.0f;
         });
+        static_for<0, R>([&](auto r) { static_for<0, S::KK>([&](auto i) { loaded(qv[r.value][i.value]); }); });
 #pragma unroll
         for (int s = 1; s < 16; s <<= 1) {
             all_lo = max(all_lo, __shfl_xor(all_lo, s));
@@ -334,27 +469,13 @@ struct Attend {
         any_hi = __builtin_amdgcn_readfirstlane(any_hi);
     }
 
-    // Table entry of the sixteen keys `u` of the sequence, and where in the page
-    // they are.  Past the sequence's end the entry is its last page's (the
-    // table's first if it has none), so that loads need no branch: a branch
-    // around a load ends in a wait for all loads before it.
-    __device__ __forceinline__ int page_entry(uint32_t u) const {
-        const uint32_t most = seq.len > 0 ? (uint32_t)(seq.len - 1) >> 4 : 0;
-        return table[(uint32_t)(min(u, most) * sh.magic >> 32)];
-    }
-    __device__ __forceinline__ uint32_t unit_in_page(uint32_t u) const { return u - (uint32_t)(u * sh.magic >> 32) * sh.units; }
-    __device__ __forceinline__ int64_t page_of(int entry) const { return (uint32_t)entry < (uint32_t)c.pages ? entry : 0; }
-    // first byte of sixteen tokens' codes (keys: their first row; values: their unit)
-    __device__ __forceinline__ int64_t unit_at(int entry, uint32_t u) const {
-        return ((page_of(entry) * c.kv_heads + h) * sh.units + unit_in_page(u)) * (16 * D);
-    }
     // the scales of this lane's sixteen keys, as loaded, and as they count:
     // scores in units of log 2, NaN for a page number that is none; past the
     // end of the sequence neither may count, whatever they are
     float ks_raw, vs_raw;
     bool bad_page;
     __device__ __forceinline__ void load_scales(int entry) {
-        const int64_t at = page_of(entry) * c.kv_heads + h;
+        const int64_t at = this->page_of(entry) * c.kv_heads + h;
         ks_raw = c.k_scale[at];
         vs_raw = c.v_scale[at];
         bad_page = (uint32_t)entry >= (uint32_t)c.pages;
@@ -406,8 +527,7 @@ struct Attend {
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
             mx = __builtin_fmaxf(m[r.value], mx * unit);
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+            mx = max_across_32(max_across_16(mx));
             if (__any(mx > m[r.value])) {
                 const float shrink = __builtin_amdgcn_exp2f(m[r.value] - mx);
                 m[r.value] = mx;
@@ -436,26 +556,9 @@ struct Attend {
         });
     }
 
-    // Values of a group where not every row sees every key.  Keys that no row
-    // sees may hold anything: their codes count as 0 (`keep` masks the others).
-    // A NaN of the others counts only for the rows that see its key, while 0 * NaN
-    // is NaN: its code becomes 0 here, and mark_nans() finds the rows that see
-    // it once the item is done.
-    bool nan_left;
-    int block_lo, block_hi, block_all_lo, block_all_hi;
-    __device__ __forceinline__ u32x4 clean(u32x4 w, u32x4 keep) {
-        uint32_t bad = 0;
-        static_for<0, 4>([&](auto x) {
-            const uint32_t v = w[x.value] & keep[x.value], n = nan_bytes(v);
-            bad |= n;
-            w[x.value] = v & ~(n * 0xffu);
-        });
-        nan_left |= bad != 0;
-        return w;
-    }
     // (a group in LDS is cleaned for all four waves' rows at once)
     __device__ __forceinline__ bool edge(int key0) const {
-        return KEYS ? key0 < all_lo || key0 + 64 > all_hi : key0 < block_all_lo || key0 + 64 > block_all_hi;
+        return KEYS ? key0 < all_lo || key0 + 64 > all_hi : this->block_edge(key0);
     }
 
     // (rare, and so key by key from memory, after the loop it would slow down)
@@ -467,7 +570,7 @@ struct Attend {
             const int key0 = key & ~63;
             if (!edge(key0) || (KEYS && ((key0 - from) / 64) % 4 != wave)) continue;
             const uint32_t u = (uint32_t)key >> 4;
-            const uint8_t* vb = (const uint8_t*)c.v + unit_at(page_entry(u), u) + 64 * g + (key & 15);
+            const uint8_t* vb = (const uint8_t*)c.v + this->unit_at(this->page_entry(u), u) + 64 * g + (key & 15);
             static_for<0, S::N>([&](auto i) {
                 static_for<0, 4>([&](auto x) {
                     if ((vb[16 * (16 * i.value + x.value)] & 0x7f) == kNaNCode) {
@@ -482,14 +585,14 @@ struct Attend {
 
     // ---- the waves share the rows
     __device__ __forceinline__ void load_keys(int key0, int entry) {
-        const uint8_t* kb = (const uint8_t*)c.k + unit_at(entry, (uint32_t)(key0 >> 4) + kg) + kr * D;
+        const uint8_t* kb = (const uint8_t*)c.k + this->unit_at(entry, (uint32_t)(key0 >> 4) + kg) + kr * D;
         static_for<0, 4>([&](auto t) {
             static_for<0, S::J>([&](auto jj) { kw[t.value][jj.value] = *(const u32x4*)(kb + 4 * t.value * D + 64 * jj.value + 16 * g); });
             if constexpr (S::REM) kx[t.value] = *(const u32x2*)(kb + 4 * t.value * D + 64 * S::J + 8 * g);
         });
     }
     __device__ __forceinline__ void load_values(int key0, int entry) {
-        const uint8_t* vb = (const uint8_t*)c.v + unit_at(entry, (uint32_t)(key0 >> 4) + g) + 16 * j;
+        const uint8_t* vb = (const uint8_t*)c.v + this->unit_at(entry, (uint32_t)(key0 >> 4) + g) + 16 * j;
         static_for<0, S::N>([&](auto i) { vw[i.value] = *(const u32x4*)(vb + i.value * 256); });
     }
 
@@ -502,8 +605,8 @@ struct Attend {
         // of the next, and V once this group's is used up.
         int k1 = 0, v1 = 0, k2 = 0, v2 = 0;
         auto entries = [&](int k0, int& k, int& v) {
-            k = page_entry((uint32_t)(k0 >> 4) + kg);
-            v = page_entry((uint32_t)(k0 >> 4) + g);
+            k = this->page_entry((uint32_t)(k0 >> 4) + kg);
+            v = this->page_entry((uint32_t)(k0 >> 4) + g);
         };
         if (key0 < end) {
             entries(key0, k1, v1);
@@ -529,7 +632,7 @@ struct Attend {
             weights(s, p, edge(key0), kv);
             if (edge(key0)) {
                 const u32x4 keep = keep_bytes(any_lo - kv, any_hi - kv);
-                static_for<0, S::N>([&](auto i) { vw[i.value] = clean(vw[i.value], keep); });
+                static_for<0, S::N>([&](auto i) { vw[i.value] = this->clean(vw[i.value], keep); });
             }
             values(p, [&](auto i) { return vw[i.value]; });
             if (more) load_values(key0 + STEP, v1);
@@ -574,7 +677,7 @@ struct Attend {
     static constexpr int L = (D + 63) / 64;
     u32x4 fk[L], fv[L];
     __device__ __forceinline__ void fetch(int key0, int entry) {
-        const int64_t at = unit_at(entry, (uint32_t)(key0 >> 4) + wave);
+        const int64_t at = this->unit_at(entry, (uint32_t)(key0 >> 4) + wave);
         static_for<0, L>([&](auto x) {
             const int i = lane + 64 * x.value;
             if (D % 64 == 0 || i < D) {
@@ -586,8 +689,8 @@ struct Attend {
     __device__ __forceinline__ void stash(int buf, int key0) {
         if (edge(key0)) {
             const int kv = key0 + 16 * wave;
-            const u32x4 keep = keep_bytes(block_lo - kv, block_hi - kv);
-            static_for<0, L>([&](auto x) { fv[x.value] = clean(fv[x.value], keep); });
+            const u32x4 keep = keep_bytes(this->block_lo - kv, this->block_hi - kv);
+            static_for<0, L>([&](auto x) { fv[x.value] = this->clean(fv[x.value], keep); });
             if (nan_left) lds.nan = 1;
         }
         static_for<0, L>([&](auto x) {
@@ -601,30 +704,19 @@ struct Attend {
     }
 
     __device__ __forceinline__ void run_rows(int from, int end) {
-        // of the workgroup's rows: both ends of what a row sees rise with it
-        {
-            const int64_t p0 = seq.len - seq.n + block / sh.group;
-            const int64_t p1 = seq.len - seq.n + (min(block + ROWS, all) - 1) / sh.group;
-            auto lower = [&](int64_t p) { return a.window && p + 1 > a.window ? (int)(p + 1 - a.window) : 0; };
-            auto upper = [&](int64_t p) { return !a.causal || p + 1 > seq.len ? seq.len : p < 0 ? 0 : (int)(p + 1); };
-            block_lo = lower(p0);
-            block_hi = upper(p1);
-            block_all_lo = lower(p1);
-            block_all_hi = upper(p0);
-        }
-        from = max(from, block_lo & ~63);
-        end = min(end, block_hi);
+        from = max(from, this->block_lo & ~63);
+        end = min(end, this->block_hi);
         __syncthreads();  // a share's last item may still be read
         if (threadIdx.x == 0) lds.nan = 0;
         __syncthreads();
         int e1 = 0, v1 = 0;  // table entries of the next group, fetched and of this lane's keys
         if (from < end) {
-            e1 = page_entry((uint32_t)(from >> 4) + wave);
-            v1 = page_entry((uint32_t)(from >> 4) + g);
+            e1 = this->page_entry((uint32_t)(from >> 4) + wave);
+            v1 = this->page_entry((uint32_t)(from >> 4) + g);
             load_scales(v1);
             fetch(from, e1);
-            e1 = page_entry((uint32_t)((from + 64) >> 4) + wave);
-            v1 = page_entry((uint32_t)((from + 64) >> 4) + g);
+            e1 = this->page_entry((uint32_t)((from + 64) >> 4) + wave);
+            v1 = this->page_entry((uint32_t)((from + 64) >> 4) + g);
             stash(0, from);
         }
         int buf = 0;
@@ -635,8 +727,8 @@ struct Attend {
             if (more) {
                 load_scales(v1);
                 const int e0 = e1;
-                e1 = page_entry((uint32_t)((key0 + 128) >> 4) + wave);
-                v1 = page_entry((uint32_t)((key0 + 128) >> 4) + g);
+                e1 = this->page_entry((uint32_t)((key0 + 128) >> 4) + wave);
+                v1 = this->page_entry((uint32_t)((key0 + 128) >> 4) + g);
                 fetch(key0 + 64, e0);
             }
             if (key0 + 64 > any_lo && key0 < any_hi) {
@@ -671,10 +763,11 @@ struct Attend {
         if (KEYS && wave > 0) return;
         const int j = here(this->j), g = here(this->g);
         static_for<0, R>([&](auto r) {
-            const int64_t row = row_of(r.value, j);
+            const int row = row_of(r.value, j);
             if (row >= all) return;
-            const int64_t tok = seq.row0 + row / sh.group;
-            const int qh = h * sh.group + (int)(row % sh.group);
+            const int place = row / sh.by_group;
+            const int64_t tok = seq.row0 + place;
+            const int qh = h * sh.group + row - place * sh.group;
             float inv = l[r.value] == 0.0f ? 0.0f : 1.0f / l[r.value];
             if (seq.poison) inv = __builtin_nanf("");
             E* y = (E*)a.out + tok * a.out_strides[0] + qh * a.out_strides[1];
@@ -694,7 +787,7 @@ struct Attend {
         if (KEYS && wave > 0) return;
         const int j = here(this->j), g = here(this->g);
         static_for<0, R>([&](auto r) {
-            const int64_t row = row_of(r.value, j);
+            const int row = row_of(r.value, j);
             if (row >= all) return;
             const int64_t at = (int64_t)slot * ROWS + (row - block);
             static_for<0, S::N>([&](auto i) { *(f32x4*)(part_o + at * D + 16 * i.value + 4 * g) = o[r.value][i.value]; });
@@ -703,24 +796,315 @@ struct Attend {
     }
 };
 
-template <class E, int D, int R, bool KEYS>
-__global__ __launch_bounds__(256, KEYS && D * R >= 256 ? 1 : 2) void attend_kernel(mfft_cache c, mfft_attend_args a, AttendShape sh,
-                                                                        float* part_o, float2* part_ml, Cut* cuts) {
-    using A = Attend<E, D, R, KEYS>;
+// Many rows: a wave has 32 of its own, as columns of v_mfma 32x32x16, and the
+// four waves of a workgroup take every group of 64 keys together.  Each wave
+// fetches sixteen keys of it, decodes them and leaves them in LDS as the
+// queries' type, so that a code is decoded once for 128 rows.
+// A lane l = 32 e + n holds, of D = A B, column n of rows 8 x + 4 e .. + 3, and
+// of A (B) contraction indices 8 e .. 8 e + 7; row 8 x + 4 e + y of the t-th of
+// the two products S^T = K Q^T is key 32 t + 16 e + 4 x + y, so that again the
+// sixteen scores of a lane are sixteen keys in order, and its weights are its
+// contraction indices of P^T.
+template <class E, int D>
+struct Tall : Item<D> {
+    using I = Item<D>;
+    using I::a, I::c, I::sh, I::seq, I::h, I::all, I::block, I::nan_left;
+    using M = Mat<E>;
+    typedef typename M::x8 x8;
+    static constexpr int ROWS = 128;
+    // keys: rows 16 bytes apart and 128 more after each sixteen, so that the
+    // sixteen rows a load takes at once (keys 0 .. 7 and 16 .. 23, or 8 .. 15
+    // and 24 .. 31) lie in different banks; values: eight tokens of a channel
+    // (16 bytes), then the next channel
+    static constexpr int KROW = 2 * D + 16, KLDS = 64 * KROW + 4 * 128, VLDS = 64 * 2 * D;
+    struct Lds {
+        uint8_t k[2][KLDS], v[2][VLDS];
+        int nan;
+    };
+    Lds& lds;
+    int lane, wave, n, e;
+
+    x8 qv[D / 16];
+    int low, top, all_lo, all_hi, any_lo, any_hi;
+    f32x16 o[D / 32];
+    float m, l;
+
+    __device__ __forceinline__ Tall(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
+        : I(c_, a_, sh_), lds(lds_) {
+        lane = threadIdx.x & 63;
+        wave = uniform((int)(threadIdx.x >> 6));
+        n = lane & 31;
+        e = lane >> 5;
+    }
+
+    __device__ __forceinline__ void begin(int b, int block_, int h_) {
+        this->take(b, block_, h_, ROWS);
+        const int n = here(this->n), e = here(this->e);
+        const int row = min(block + 32 * wave + n, all - 1);
+        const int tok = row / sh.by_group;
+        const int qh = h * sh.group + row - tok * sh.group;
+        const E* q = (const E*)a.q + (seq.row0 + tok) * a.q_strides[0] + qh * a.q_strides[1] + 8 * e;
+        static_for<0, D / 16>([&](auto i) { qv[i.value] = *(const x8*)(q + 16 * i.value); });
+        low = this->lower(tok);
+        top = max(this->upper(tok), low);
+        all_lo = any_lo = low;
+        all_hi = any_hi = top;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            all_lo = max(all_lo, __shfl_xor(all_lo, s));
+            all_hi = min(all_hi, __shfl_xor(all_hi, s));
+            any_lo = min(any_lo, __shfl_xor(any_lo, s));
+            any_hi = max(any_hi, __shfl_xor(any_hi, s));
+        }
+        all_lo = uniform(all_lo);
+        all_hi = uniform(all_hi);
+        any_lo = uniform(any_lo);
+        any_hi = uniform(any_hi);
+        static_for<0, D / 32>([&](auto i) { static_for<0, 16>([&](auto x) { o[i.value][x.value] = 0.0f; }); });
+        m = kLowest;
+        l = 0.0f;
+        static_for<0, D / 16>([&](auto i) { loaded(qv[i.value]); });
+    }
+
+    static constexpr int L = (D + 63) / 64;
+    u32x4 fk[L], fv[L];
+    float fvs;  // value scale of the sixteen keys this wave fetches
+    __device__ __forceinline__ void fetch(int key0, int entry) {
+        const uint32_t u = (uint32_t)(key0 >> 4) + wave;
+        const int64_t at = this->unit_at(entry, u);
+        static_for<0, L>([&](auto x) {
+            const int i = lane + 64 * x.value;
+            if (D % 64 == 0 || i < D) {
+                fk[x.value] = *(const u32x4*)((const uint8_t*)c.k + at + 16 * i);
+                fv[x.value] = *(const u32x4*)((const uint8_t*)c.v + at + 16 * i);
+            }
+        });
+        fvs = c.v_scale[this->page_of(entry) * c.kv_heads + h];
+    }
+    __device__ __forceinline__ void stash(int buf, int key0) {
+        if (this->block_edge(key0)) {
+            const int kv = key0 + 16 * wave;
+            const u32x4 keep = keep_bytes(this->block_lo - kv, this->block_hi - kv);
+            static_for<0, L>([&](auto x) { fv[x.value] = this->clean(fv[x.value], keep); });
+            if (nan_left) lds.nan = 1;
+        }
+        // a page that is none, or the stand-in past the end, may have any scale
+        const float vs = key0 + 16 * wave < seq.len ? fvs : 1.0f;
+        static_for<0, L>([&](auto x) {
+            const int i = lane + 64 * x.value;
+            if (D % 64 == 0 || i < D) {
+                const int row = i / (D / 16), at = i % (D / 16);
+                uint8_t* k = lds.k[buf] + (16 * wave + row) * KROW + 128 * wave + 32 * at;
+                *(x8*)k = decode8<E>(fk[x.value][0], fk[x.value][1], 1.0f);
+                *(x8*)(k + 16) = decode8<E>(fk[x.value][2], fk[x.value][3], 1.0f);
+                uint8_t* v = lds.v[buf] + (wave * D + i) * 16;
+                *(x8*)v = decode8<E>(fv[x.value][0], fv[x.value][1], vs);
+                *(x8*)(v + 4 * D * 16) = decode8<E>(fv[x.value][2], fv[x.value][3], vs);
+            }
+        });
+    }
+
+    // scales of the keys of this lane's scores, as Attend's load_scales
+    float ks_raw[2], cs[2];
+    bool bad_page[2];
+    __device__ __forceinline__ void load_scales(const int (&entry)[2]) {
+        static_for<0, 2>([&](auto t) {
+            ks_raw[t.value] = c.k_scale[this->page_of(entry[t.value]) * c.kv_heads + h];
+            bad_page[t.value] = (uint32_t)entry[t.value] >= (uint32_t)c.pages;
+        });
+    }
+
+    __device__ __forceinline__ void weights(f32x16 (&s)[2], x8 (&p)[4], bool at_edge, int key0) {
+        float unit[2] = {cs[0], cs[1]};
+        if (at_edge) {
+            static_for<0, 2>([&](auto t) {
+                const int kv = key0 + 32 * t.value + 16 * e;
+                const int lo = min(max(low - kv, 0), 16), hi = min(max(top - kv, 0), 16);
+                const int seen = (int)((1u << hi) - (1u << lo));
+                static_for<0, 16>([&](auto i) {
+                    const uint32_t bit = (uint32_t)((seen << (31 - i.value)) >> 31);
+                    const uint32_t v = __float_as_uint(s[t.value][i.value] * cs[t.value]);
+                    s[t.value][i.value] = __uint_as_float((v & bit) | (0xff800000u & ~bit));
+                });
+                unit[t.value] = 1.0f;
+            });
+        }
+        float mx = m;
+        static_for<0, 2>([&](auto t) {
+            float x = s[t.value][0];
+            static_for<1, 16>([&](auto i) { x = __builtin_fmaxf(x, s[t.value][i.value]); });
+            mx = __builtin_fmaxf(mx, x * unit[t.value]);
+        });
+        mx = max_across_32(mx);
+        if (__any(mx > m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - mx);
+            m = mx;
+            l *= shrink;
+            static_for<0, D / 32>([&](auto i) { o[i.value] *= shrink; });
+        }
+        static_for<0, 2>([&](auto t) {
+            static_for<0, 16>([&](auto i) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t.value][i.value], unit[t.value], -m));
+                l += w;
+                p[2 * t.value + i.value / 8][i.value % 8] = (E)w;
+            });
+        });
+    }
+
+    __device__ __forceinline__ void run(int from, int end) {
+        from = max(from, this->block_lo & ~63);
+        end = min(end, this->block_hi);
+        __syncthreads();  // a share's last item may still be read
+        if (threadIdx.x == 0) lds.nan = 0;
+        __syncthreads();
+        int e1 = 0, k1[2] = {0, 0};  // table entries of the next group, fetched and of this lane's keys
+        auto entries = [&](int key0) {
+            e1 = this->page_entry((uint32_t)(key0 >> 4) + wave);
+            k1[0] = this->page_entry((uint32_t)(key0 >> 4) + e);
+            k1[1] = this->page_entry((uint32_t)(key0 >> 4) + 2 + e);
+        };
+        if (from < end) {
+            entries(from);
+            load_scales(k1);
+            fetch(from, e1);
+            entries(from + 64);
+            stash(0, from);
+        }
+        // of K: row n of a product, see above
+        const int key_row = 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3);
+        const int k_at = key_row * KROW + 128 * ((n >> 2) & 1) + 16 * e, v_at = (e * D + n) * 16;
+        int buf = 0;
+        for (int key0 = from; key0 < end; key0 += 64) {
+            __syncthreads();
+            const bool more = key0 + 64 < end;
+            static_for<0, 2>([&](auto t) {
+                cs[t.value] = bad_page[t.value] ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw[t.value];
+            });
+            if (more) {
+                load_scales(k1);
+                const int e0 = e1;
+                entries(key0 + 128);
+                fetch(key0 + 64, e0);
+            }
+            if (key0 + 64 > any_lo && key0 < any_hi) {
+                f32x16 s[2];
+                x8 p[4];
+                const uint8_t* kb = lds.k[buf] + k_at;
+                static_for<0, 2>([&](auto t) {
+                    static_for<0, 16>([&](auto x) { s[t.value][x.value] = 0.0f; });
+                    static_for<0, D / 16>([&](auto i) {
+                        const x8 k = *(const x8*)(kb + t.value * (32 * KROW + 256) + 32 * i.value);
+                        s[t.value] = M::mfma(k, qv[i.value], s[t.value]);
+                    });
+                });
+                weights(s, p, key0 < all_lo || key0 + 64 > all_hi, key0);
+                const uint8_t* vb = lds.v[buf] + v_at;
+                static_for<0, D / 32>([&](auto i) {
+                    static_for<0, 4>([&](auto x) {  // product x: keys 32 (x / 2) + 16 e + 8 (x % 2) and on
+                        const x8 v = *(const x8*)(vb + (((x.value % 2) * 4 + 2 * (x.value / 2)) * D + 32 * i.value) * 16);
+                        o[i.value] = M::mfma(v, p[x.value], o[i.value]);
+                    });
+                });
+            }
+            buf ^= 1;
+            if (more) stash(buf, key0 + 64);
+        }
+        __syncthreads();
+        nan_left = lds.nan != 0;
+        mark_nans(from, end);
+        l += __shfl_xor(l, 32);
+    }
+
+    __device__ __forceinline__ void mark_nans(int from, int end) {
+        if (!__any(nan_left)) return;
+        const int e = here(this->e);
+#pragma unroll 1
+        for (int key = from; key < end; ++key) {
+            if (!this->block_edge(key & ~63)) continue;
+            const uint32_t u = (uint32_t)key >> 4;
+            const uint8_t* vb = (const uint8_t*)c.v + this->unit_at(this->page_entry(u), u) + 64 * e + (key & 15);
+            const bool seen = key >= low && key < top;
+            static_for<0, D / 32>([&](auto i) {
+                static_for<0, 16>([&](auto x) {
+                    if ((vb[16 * (32 * i.value + 8 * (x.value / 4) + x.value % 4)] & 0x7f) == kNaNCode && seen)
+                        o[i.value][x.value] = __builtin_nanf("");
+                });
+            });
+        }
+    }
+
+    __device__ __forceinline__ void store() const {
+        const int n = here(this->n), e = here(this->e);
+        const int row = block + 32 * wave + n;
+        if (row >= all) return;
+        const int place = row / sh.by_group;
+        const int64_t tok = seq.row0 + place;
+        const int qh = h * sh.group + row - place * sh.group;
+        float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (seq.poison) inv = __builtin_nanf("");
+        E* y = (E*)a.out + tok * a.out_strides[0] + qh * a.out_strides[1] + 4 * e;
+        static_for<0, D / 32>([&](auto i) {
+            static_for<0, 4>([&](auto x) {
+                union {
+                    E e[4];
+                    u32x2 w;
+                } u;
+                static_for<0, 4>([&](auto z) { u.e[z.value] = (E)(o[i.value][4 * x.value + z.value] * inv); });
+                *(u32x2*)(y + 32 * i.value + 8 * x.value) = u.w;
+            });
+        });
+        if (a.lse && e == 0) a.lse[tok * a.q_heads + qh] = log_sum(m, l, seq.poison);
+    }
+    __device__ __forceinline__ void store_part(int slot, float* part_o, float2* part_ml) const {
+        const int n = here(this->n), e = here(this->e);
+        if (block + 32 * wave + n >= all) return;
+        const int64_t at = (int64_t)slot * ROWS + 32 * wave + n;
+        static_for<0, D / 32>([&](auto i) {
+            static_for<0, 4>([&](auto x) {
+                f32x4 w;
+                static_for<0, 4>([&](auto z) { w[z.value] = o[i.value][4 * x.value + z.value]; });
+                *(f32x4*)(part_o + at * D + 32 * i.value + 8 * x.value + 4 * e) = w;
+            });
+        });
+        if (e == 0) part_ml[at] = make_float2(m, l);
+    }
+};
+
+// The forms and the workgroups that a CU holds at once, by their registers and
+// LDS: O and Q are D R / 4 + D R / 8 registers a lane, and kKeys holds K and V
+// of the next group too.
+enum Form { kKeys1, kKeys2, kKeys4, kRows, kTall };
+constexpr int attend_per_cu(int d, Form f) {
+    return f == kKeys1 ? (d >= 256 ? 1 : 2) : f == kKeys2 ? (d >= 128 ? 1 : 2) : f == kKeys4 ? 1 : 2;
+}
+template <class E, int D, Form F>
+struct FormOf {
+    typedef Attend<E, D, F == kKeys4 ? 4 : F == kKeys2 ? 2 : 1, F != kRows> type;
+};
+template <class E, int D>
+struct FormOf<E, D, kTall> {
+    typedef Tall<E, D> type;
+};
+
+template <class E, int D, Form F>
+__global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_cache c, mfft_attend_args a, AttendShape sh,
+                                                                          float* part_o, float2* part_ml, Cut* cuts) {
+    using A = typename FormOf<E, D, F>::type;
     __shared__ __align__(16) typename A::Lds lds;
     A w(c, a, sh, lds);
     // groups [at, stop) of the list; with one workgroup an item, of that item
     int64_t before, at = 0, stop, share = INT64_MAX;
     int b, item, tile = 0;
     if (sh.grid == 0) {
-        b = locate(c, a, sh, true, blockIdx.x, before);
+        b = WorkList{c, a, sh, true, 0, 0}.find(blockIdx.x, before, false);
         if (b < 0) return;
         w.seq = sequence(c, a, sh, b);
         item = (int)((int64_t)blockIdx.x - before);
         stop = w.seq.tiles;
     } else {
-        const int64_t total = all_work(c, a, sh);
-        const int64_t even = (total + sh.grid - 1) / sh.grid;
+        WorkList list{c, a, sh, false, 0, 0};
+        const int64_t total = list.total();
+        const int64_t even = quotient(total + sh.grid - 1, sh.grid);
         share = even > sh.least ? even : sh.least;
         at = blockIdx.x * share;
         stop = at + share < total ? at + share : total;
@@ -728,22 +1112,26 @@ __global__ __launch_bounds__(256, KEYS && D * R >= 256 ? 1 : 2) void attend_kern
             if (threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
             return;
         }
-        b = locate(c, a, sh, false, at, before);
+        b = list.find(at, before, a.sequences <= 64);
         w.seq = sequence(c, a, sh, b);
-        item = uniform((int)((at - before) / w.seq.tiles));
-        tile = uniform((int)((at - before) - (int64_t)item * w.seq.tiles));
+        const int64_t i = quotient(at - before, w.seq.tiles);
+        item = (int)i;
+        tile = (int)(at - before - i * w.seq.tiles);
     }
     Cut cut{0, 0, 0, 0};
     while (true) {
         const int upto = stop - at < w.seq.tiles - tile ? tile + (int)(stop - at) : w.seq.tiles;
-        const int block = item / c.kv_heads, h = item % c.kv_heads;
+        const int block = item / sh.by_heads, h = item - block * c.kv_heads;
         w.begin(b, block, h);
         w.run(w.seq.low + 64 * tile, w.seq.low + 64 * upto);
         if (tile == 0 && upto == w.seq.tiles) {
             w.store();
         } else {
             w.store_part(2 * (int)blockIdx.x + (tile == 0 ? 1 : 0), part_o, part_ml);
-            if (tile == 0) cut = {(int)((at + w.seq.tiles - 1) / share) - (int)blockIdx.x + 1, b, block, h};
+            if (tile == 0) {  // its last group lies `past` groups past this share's end
+                const int past = (int)(at + w.seq.tiles - 1 - stop);
+                cut = {share > past ? 2 : past / (int)share + 2, b, block, h};
+            }
         }
         at += upto - tile;
         if (at >= stop) break;
@@ -758,59 +1146,69 @@ __global__ __launch_bounds__(256, KEYS && D * R >= 256 ? 1 : 2) void attend_kern
     if (sh.grid && threadIdx.x == 0) cuts[blockIdx.x] = cut;
 }
 
-// A cut item's row: one workgroup, its waves every fourth part, each lane
-// D / 64 channels.
+// Cut items, `sh.join_rows` rows a workgroup: of few parts, a wave a row; of
+// many, all four waves every fourth part of one row after the other.  Each lane
+// takes D / 64 channels.
 template <class E, int D>
 __global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_args a, AttendShape sh, const float* part_o,
                                                    const float2* part_ml, const Cut* cuts) {
     constexpr int C = (D + 63) / 64;
-    const int share = blockIdx.x / sh.live, row_in = blockIdx.x % sh.live;
+    const int groups = (sh.live + sh.join_rows - 1) / sh.join_rows;
+    const int share = blockIdx.x / groups;
     const Cut cut = cuts[share];
     if (cut.parts == 0) return;
     const Sequence seq = sequence(c, a, sh, cut.b);
-    const int64_t row = (int64_t)cut.block * sh.rows + row_in;
-    if (row >= seq.n * sh.group) return;
+    const int block = cut.block * sh.rows, all = seq.n * sh.group;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    auto slot = [&](int p) { return (int64_t)(2 * (share + p) + (p == 0 ? 1 : 0)) * sh.rows + row_in; };
+    const bool wide = cut.parts > 8;
+    const int first = (int)(blockIdx.x % groups) * sh.join_rows;
+    const int end = min(min(first + sh.join_rows, sh.live), all - block);
+    __shared__ float sl[4], so[4][64 * C];
 
-    float m = kLowest;
-    for (int p = lane; p < cut.parts; p += 64) m = __builtin_fmaxf(m, part_ml[slot(p)].x);
-    m = wave_max(m);
-    float l = 0.0f, o[C] = {};
-#pragma unroll 4
-    for (int p = wave; p < cut.parts; p += 4) {
-        const int64_t s = slot(p);
-        const float2 ml = part_ml[s];
-        const float f = __builtin_amdgcn_exp2f(ml.x - m);
-        l += ml.y * f;
+    for (int row = first + (wide ? 0 : wave); row < end; row += wide ? 1 : 4) {
+        auto slot = [&](int p) { return (int64_t)(2 * (share + p) + (p == 0 ? 1 : 0)) * sh.rows + row; };
+        float m = kLowest;
+        for (int p = lane; p < cut.parts; p += 64) m = __builtin_fmaxf(m, part_ml[slot(p)].x);
+        m = wave_max(m);
+        float l = 0.0f, o[C] = {};
+#pragma unroll 8
+        for (int p = wide ? wave : 0; p < cut.parts; p += wide ? 4 : 1) {
+            const int64_t s = slot(p);
+            const float2 ml = part_ml[s];
+            const float f = __builtin_amdgcn_exp2f(ml.x - m);
+            l += ml.y * f;
+#pragma unroll
+            for (int x = 0; x < C; ++x)
+                if (D % 64 == 0 || lane + 64 * x < D) o[x] += part_o[s * D + lane + 64 * x] * f;
+        }
+        if (wide) {
+            __syncthreads();
+            if (lane == 0) sl[wave] = l;
+#pragma unroll
+            for (int x = 0; x < C; ++x) so[wave][lane + 64 * x] = o[x];
+            __syncthreads();
+            if (wave > 0) continue;
+            l = sl[0] + sl[1] + sl[2] + sl[3];
+#pragma unroll
+            for (int x = 0; x < C; ++x) o[x] = so[0][lane + 64 * x] + so[1][lane + 64 * x] + so[2][lane + 64 * x] + so[3][lane + 64 * x];
+        }
+        float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (seq.poison) inv = __builtin_nanf("");
+        const int place = (block + row) / sh.by_group;
+        const int64_t tok = seq.row0 + place;
+        const int qh = cut.h * sh.group + block + row - place * sh.group;
+        E* y = (E*)a.out + tok * a.out_strides[0] + qh * a.out_strides[1];
 #pragma unroll
         for (int x = 0; x < C; ++x)
-            if (D % 64 == 0 || lane + 64 * x < D) o[x] += part_o[s * D + lane + 64 * x] * f;
+            if (D % 64 == 0 || lane + 64 * x < D) y[lane + 64 * x] = (E)(o[x] * inv);
+        if (a.lse && lane == 0) a.lse[tok * a.q_heads + qh] = log_sum(m, l, seq.poison);
     }
-    __shared__ float sl[4], so[4][64 * C];
-    if (lane == 0) sl[wave] = l;
-#pragma unroll
-    for (int x = 0; x < C; ++x) so[wave][lane + 64 * x] = o[x];
-    __syncthreads();
-    l = sl[0] + sl[1] + sl[2] + sl[3];
-    float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (seq.poison) inv = __builtin_nanf("");
-    const int64_t tok = seq.row0 + row / sh.group;
-    const int qh = cut.h * sh.group + (int)(row % sh.group);
-    E* y = (E*)a.out + tok * a.out_strides[0] + qh * a.out_strides[1];
-    if (threadIdx.x < D)
-        y[threadIdx.x] = (E)((so[0][threadIdx.x] + so[1][threadIdx.x] + so[2][threadIdx.x] + so[3][threadIdx.x]) * inv);
-    if (a.lse && threadIdx.x == 0) a.lse[tok * a.q_heads + qh] = log_sum(m, l, seq.poison);
 }
 
 // ---- the launch ---------------------------------------------------------------
-constexpr int kShares = 512;    // two workgroups on each of 256 CUs
-constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
-
 struct AttendLaunch {
     AttendShape sh;
-    int r;            // row tiles of a wave
-    bool keys;
+    Form form;
     int64_t grid, o_bytes, ml_bytes, cut_bytes;
 };
 
@@ -820,21 +1218,30 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a) {
     w.sh.units = c.page_size / 16;
     w.sh.magic = ((uint64_t)1 << 32) / w.sh.units + 1;
     w.sh.per = a.offsets ? 1 : a.tokens / a.sequences;
-    w.sh.least = kLeastTiles;
     // rows of a sequence and key head, on average where there are offsets
     const int64_t rows = (a.tokens * w.sh.group + a.sequences - 1) / a.sequences;
-    w.keys = rows <= 32;
-    w.r = w.keys ? (rows <= 16 ? 1 : 2) : (rows <= 64 || c.head_dim > 128 ? 1 : 2);
-    w.sh.rows = w.keys ? 16 * w.r : 64 * w.r;
+    const int D = c.head_dim;
+    w.form = rows <= 16 ? kKeys1 : rows <= 32 && D <= 128 ? kKeys2 : rows <= 64 && D <= 96 ? kKeys4 : rows <= 64 || D > 128 ? kRows : kTall;
+    w.sh.rows = w.form == kKeys1 ? 16 : w.form == kKeys2 ? 32 : w.form == kTall ? 128 : 64;
+    // a cut costs its rows' partial sums, written and read again: about a
+    // quarter as many groups of keys as it has rows
+    w.sh.least = w.sh.rows / 4 > kLeastTiles ? w.sh.rows / 4 : kLeastTiles;
+    w.sh.log_rows = ilog2(w.sh.rows);
+    w.sh.by_group = divisor(w.sh.group);
+    w.sh.by_heads = divisor(c.kv_heads);
     w.sh.live = !a.offsets && rows < w.sh.rows ? (int)rows : w.sh.rows;
     const int64_t items = (a.tokens * w.sh.group / w.sh.rows + a.sequences) * c.kv_heads;  // at most
     const bool whole = a.max_length && a.max_length <= kLeastTiles * 64;
-    w.sh.grid = whole ? 0 : kShares;
-    w.grid = whole ? items : kShares;
+    w.grid = items;
     if (!whole) {
-        w.o_bytes = (int64_t)2 * kShares * w.sh.rows * c.head_dim * 4;
-        w.ml_bytes = (int64_t)2 * kShares * w.sh.rows * 8;
-        w.cut_bytes = kShares * sizeof(Cut);
+        // as many shares as workgroups run at once
+        w.sh.grid = kCUs * attend_per_cu(D, w.form);
+        w.grid = w.sh.grid;
+        // few sequences and heads: their items are cut into many parts
+        w.sh.join_rows = w.sh.live <= 16 && w.sh.grid >= 8 * (int64_t)a.sequences * c.kv_heads ? 1 : w.sh.live > 16 ? 8 : 4;
+        w.o_bytes = (int64_t)2 * w.sh.grid * w.sh.rows * D * 4;
+        w.ml_bytes = (int64_t)2 * w.sh.grid * w.sh.rows * 8;
+        w.cut_bytes = w.sh.grid * sizeof(Cut);
     }
     return w;
 }
@@ -845,13 +1252,16 @@ void launch_dim(const mfft_cache& c, const mfft_attend_args& a, const AttendLaun
     float2* ml = (float2*)((char*)a.workspace + w.o_bytes);
     Cut* cuts = (Cut*)((char*)ml + w.ml_bytes);
     const uint32_t grid = (uint32_t)w.grid;
-    if (w.keys && w.r == 1) attend_kernel<E, D, 1, true><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
-    else if (w.keys) attend_kernel<E, D, 2, true><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
-    else if (w.r == 1) attend_kernel<E, D, 1, false><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
-    else if constexpr (D <= 128) attend_kernel<E, D, 2, false><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+    if (w.form == kKeys1) attend_kernel<E, D, kKeys1><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+    else if (w.form == kRows) attend_kernel<E, D, kRows><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+    else if constexpr (D <= 128) {
+        if (w.form == kKeys2) attend_kernel<E, D, kKeys2><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+        else if (w.form == kTall) attend_kernel<E, D, kTall><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+        else if constexpr (D <= 96) attend_kernel<E, D, kKeys4><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+    }
     mark(s);
     if (w.sh.grid) {
-        join_kernel<E, D><<<kShares * w.sh.live, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+        join_kernel<E, D><<<w.sh.grid * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows), 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
         mark(s);
     }
 }

@@ -269,8 +269,11 @@ static int check_attend(const mfft_cache* c, const mfft_attend_args* a) {
                     (long long)a->tokens, a->sequences);
     if (a->q_heads < 1 || a->q_heads % c->kv_heads || a->q_heads > 65536)
         return fail(MFFT_ERR_VALUE, "q_heads must be a multiple of the cache's %d heads, at most 65536, got %d", c->kv_heads, a->q_heads);
+    if (a->tokens > ((int64_t)1 << 30) / a->q_heads)
+        return fail(MFFT_ERR_UNSUPPORTED, "more than 2^30 query rows (%lld tokens of %d heads); split the call",
+                    (long long)a->tokens, a->q_heads);
     if (!std::isfinite(a->scale) || a->scale < 0.0f) return fail(MFFT_ERR_VALUE, "scale must be finite and not negative");
-    if (a->window < 0 || a->window > 0x7fffffff) return fail(MFFT_ERR_VALUE, "window must be in [0, 2^31)");
+    if (a->window < 0 || a->window > (int64_t)1 << 30) return fail(MFFT_ERR_VALUE, "window must be in [0, 2^30]");
     if ((int64_t)a->table_width * c->page_size > (int64_t)1 << 30)
         return fail(MFFT_ERR_VALUE, "page_table holds more than 2^30 positions a sequence");
     if (a->max_length < 0) return fail(MFFT_ERR_VALUE, "max_length must not be negative");
