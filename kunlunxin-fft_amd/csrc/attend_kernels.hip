@@ -20,6 +20,8 @@
 //
 // Codes become the queries' type exactly (e4m3 fits both); V's power-of-two
 // scale goes in with the conversion, K's into the 32-bit score.
+#include <algorithm>
+
 #include "lm_device.hpp"
 #include "mfft_device.hpp"
 
@@ -165,6 +167,11 @@ struct AttendShape {
 
 constexpr int kCUs = 256;
 constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
+// Up to here, times the items there are for each workgroup at once, an item is
+// never cut: the second launch costs more than it saves, and many items balance
+// by themselves.  One token of one sequence of 1000: 10.7 us whole, 15.1 cut;
+// 256 sequences of up to 1000, mixed: 55 and 111 us.
+constexpr int kWholeTiles = 16;
 
 // the item that starts in share i and is cut at its end: its parts are in
 // slots 2 i + 1, 2 (i + 1), 2 (i + 2), ... of the workspace
@@ -1231,11 +1238,15 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a) {
     w.sh.by_heads = divisor(c.kv_heads);
     w.sh.live = !a.offsets && rows < w.sh.rows ? (int)rows : w.sh.rows;
     const int64_t items = (a.tokens * w.sh.group / w.sh.rows + a.sequences) * c.kv_heads;  // at most
-    const bool whole = a.max_length && a.max_length <= kLeastTiles * 64;
+    const int64_t at_once = kCUs * attend_per_cu(D, w.form);
+    const int64_t table = (int64_t)a.table_width * c.page_size;
+    const int64_t longest = a.max_length && a.max_length < table ? a.max_length : table;
+    const int64_t each = std::max<int64_t>(1, std::max<int64_t>(a.sequences, a.tokens * w.sh.group / w.sh.rows) * c.kv_heads / at_once);
+    const bool whole = longest <= 64 * kWholeTiles * each;
     w.grid = items;
     if (!whole) {
         // as many shares as workgroups run at once
-        w.sh.grid = kCUs * attend_per_cu(D, w.form);
+        w.sh.grid = (int)at_once;
         w.grid = w.sh.grid;
         // few sequences and heads: their items are cut into many parts
         w.sh.join_rows = w.sh.live <= 16 && w.sh.grid >= 8 * (int64_t)a.sequences * c.kv_heads ? 1 : w.sh.live > 16 ? 8 : 4;
