@@ -27,8 +27,8 @@ struct AppendGrid {
     int q_heads;         // heads of a piece
 };
 
-// Query heads a thread takes: sixteen, or as few as it takes to have 2^15
-// threads (a wave on each of 1024 SIMDs, half of them twice).
+// Query heads a thread takes: sixteen, or as few as it takes to have 2^18
+// threads (four waves on each of 1024 SIMDs).
 constexpr int kQueryHeads = 16;
 
 __host__ __device__ inline AppendGrid append_grid(const mfft_cache& c, const mfft_append_args& a, int v) {
@@ -38,7 +38,7 @@ __host__ __device__ inline AppendGrid append_grid(const mfft_cache& c, const mff
     // v pairs (2 v channels) of a token and piece of the heads a thread
     const int64_t chunks = a.tokens * (c.head_dim / (2 * v));
     g.q_heads = 1;
-    while (v > 1 && g.q_heads < kQueryHeads && g.q_heads < a.q_heads && chunks * a.q_heads > ((int64_t)1 << 15) * g.q_heads) g.q_heads *= 2;
+    while (v > 1 && g.q_heads < kQueryHeads && g.q_heads < a.q_heads && chunks * a.q_heads > ((int64_t)1 << 18) * g.q_heads) g.q_heads *= 2;
     g.q_slabs = a.q ? (a.q_heads + g.q_heads - 1) / g.q_heads : 0;
     g.q_blocks = (chunks * g.q_slabs + 255) / 256;
     return g;
