@@ -42,7 +42,20 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kLowest = -1e30f;  // start of the running maximum: no score seen
+constexpr float kLowest = -3.402823466e38f;  // start of the running maximum: no score seen
+
+// Up to here (in units of log 2) a score less its row's maximum is one fma of
+// the unscaled score, whose maximum alone is rounded: off by half a unit of
+// the maximum's last place, 2^-4 at most.  Past it that unit grows until the
+// largest weight is no number; scores are then rounded before the difference,
+// as the maximum is.
+constexpr float kFusedScores = 1048576.0f;
+
+// a b, rounded whatever is done with it
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 
 // ---- the two query types ----------------------------------------------------
 template <class E>
@@ -423,6 +436,7 @@ struct Attend : Item<D> {
     int all_lo, all_hi, any_lo, any_hi;  // and all, and any, of the wave's rows
     f32x4 o[R][S::N];
     float m[R], l[R];
+    bool large;                        // some row's maximum has been past kFusedScores
 
     // of the group at hand
     u32x4 kw[4][S::J > 0 ? S::J : 1];
@@ -448,6 +462,7 @@ struct Attend : Item<D> {
         all_hi = seq.len;
         any_lo = seq.len;
         any_hi = 0;
+        large = false;
         const int j = here(this->j), g = here(this->g);
         static_for<0, R>([&](auto r) {
             const int row = min(row_of(r.value, j), all - 1);  // rows past the last repeat it and are not stored
@@ -524,8 +539,8 @@ struct Attend : Item<D> {
 
     // P from S, m and l moved on, O rescaled where m grew
     __device__ __forceinline__ void weights(f32x4 (&s)[R][4], x8 (&p)[R][2], bool at_edge, int kv) {
+        const float unit = at_edge ? 1.0f : cs;
         static_for<0, R>([&](auto r) {
-            float unit = cs;
             if (at_edge) {
                 // bit i: key kv + i is seen; as masks of whole words, which
                 // take no condition registers
@@ -536,7 +551,6 @@ struct Attend : Item<D> {
                     const uint32_t v = __float_as_uint(s[r.value][i.value / 4][i.value % 4] * cs);
                     s[r.value][i.value / 4][i.value % 4] = __uint_as_float((v & bit) | (0xff800000u & ~bit));
                 });
-                unit = 1.0f;
             }
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
@@ -545,11 +559,25 @@ struct Attend : Item<D> {
             if (__any(mx > m[r.value])) {
                 const float shrink = __builtin_amdgcn_exp2f(m[r.value] - mx);
                 m[r.value] = mx;
+                large |= __any(__builtin_fabsf(mx) > kFusedScores && mx > kLowest);
                 l[r.value] *= shrink;
                 static_for<0, S::N>([&](auto i) { o[r.value][i.value] *= shrink; });
             }
+        });
+        float from[R], by = unit;
+        static_for<0, R>([&](auto r) { from[r.value] = -m[r.value]; });
+        if (large) {
+            static_for<0, R>([&](auto r) {
+                static_for<0, 16>([&](auto i) {
+                    s[r.value][i.value / 4][i.value % 4] = product(s[r.value][i.value / 4][i.value % 4], unit) - m[r.value];
+                });
+                from[r.value] = 0.0f;
+            });
+            by = 1.0f;
+        }
+        static_for<0, R>([&](auto r) {
             static_for<0, 16>([&](auto i) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r.value][i.value / 4][i.value % 4], unit, -m[r.value]));
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r.value][i.value / 4][i.value % 4], by, from[r.value]));
                 l[r.value] += w;
                 p[r.value][i.value / 8][i.value % 8] = (E)w;
             });
@@ -841,6 +869,7 @@ struct Tall : Item<D> {
     int low, top, all_lo, all_hi, any_lo, any_hi;
     f32x16 o[D / 32];
     float m, l;
+    bool large;  // some row's maximum has been past kFusedScores
 
     __device__ __forceinline__ Tall(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
         : I(c_, a_, sh_), lds(lds_) {
@@ -876,6 +905,7 @@ struct Tall : Item<D> {
         static_for<0, D / 32>([&](auto i) { static_for<0, 16>([&](auto x) { o[i.value][x.value] = 0.0f; }); });
         m = kLowest;
         l = 0.0f;
+        large = false;
         static_for<0, D / 16>([&](auto i) { loaded(qv[i.value]); });
     }
 
@@ -952,12 +982,21 @@ struct Tall : Item<D> {
         if (__any(mx > m)) {
             const float shrink = __builtin_amdgcn_exp2f(m - mx);
             m = mx;
+            large |= __any(__builtin_fabsf(m) > kFusedScores && m > kLowest);
             l *= shrink;
             static_for<0, D / 32>([&](auto i) { o[i.value] *= shrink; });
         }
+        float from = -m;
+        if (large) {
+            static_for<0, 2>([&](auto t) {
+                static_for<0, 16>([&](auto i) { s[t.value][i.value] = product(s[t.value][i.value], unit[t.value]) - m; });
+                unit[t.value] = 1.0f;
+            });
+            from = 0.0f;
+        }
         static_for<0, 2>([&](auto t) {
             static_for<0, 16>([&](auto i) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t.value][i.value], unit[t.value], -m));
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t.value][i.value], unit[t.value], from));
                 l += w;
                 p[2 * t.value + i.value / 8][i.value % 8] = (E)w;
             });
