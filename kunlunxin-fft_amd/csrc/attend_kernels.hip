@@ -3,7 +3,8 @@
 // One pass over the keys a row of queries sees, with a running maximum m and
 // sum l of exponentials: for each 64 keys s = scale * K q, m' = max(m, s),
 // p = 2^(s - m'), l = l 2^(m - m') + sum p, O = O 2^(m - m') + V p, and
-// out = O / l at the end (s in units of log 2).
+// out = O / l at the end (s in units of log 2; in float16 m is kept 14 lower,
+// see Mat).
 //
 // Both products run on the matrix cores with queries as columns: S^T = K Q^T
 // and O^T = V^T P^T, sixteen rows of queries (the query heads of one key head,
@@ -58,6 +59,13 @@ __device__ __forceinline__ float product(float a, float b) {
 }
 
 // ---- the two query types ----------------------------------------------------
+// `offset`: what a row's weights are relative to, 2^(s - offset), from its
+// largest score x.  l and O are relative to the same and out = O / l, so any
+// offset gives the same row; m below is the offset.  In float16, whose least
+// step is 2^-24, weights reach 2^13 to 2^14 instead of 1, so that those 2^-25
+// to 2^-38 of the largest, which l counts, are not lost from O.  (A whole
+// number, so that nothing is rounded; past kFusedScores, where 14 would be,
+// the largest score itself.)
 template <class E>
 struct Mat;
 template <>
@@ -74,6 +82,7 @@ struct Mat<__bf16> {
     static __device__ __forceinline__ x2 decode(uint32_t w, float scale) {
         return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
     }
+    static __device__ __forceinline__ float offset(float x) { return x; }
 };
 template <>
 struct Mat<_Float16> {
@@ -88,6 +97,9 @@ struct Mat<_Float16> {
     template <bool HI>
     static __device__ __forceinline__ x2 decode(uint32_t w, float scale) {
         return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI);
+    }
+    static __device__ __forceinline__ float offset(float x) {
+        return __builtin_fabsf(x) <= kFusedScores ? __builtin_ceilf(x) - 14.0f : x;
     }
 };
 
@@ -554,8 +566,7 @@ struct Attend : Item<D> {
             }
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
-            mx = __builtin_fmaxf(m[r.value], mx * unit);
-            mx = max_across_32(max_across_16(mx));
+            mx = __builtin_fmaxf(m[r.value], M::offset(max_across_32(max_across_16(mx * unit))));
             if (__any(mx > m[r.value])) {
                 const float shrink = __builtin_amdgcn_exp2f(m[r.value] - mx);
                 m[r.value] = mx;
@@ -972,13 +983,13 @@ struct Tall : Item<D> {
                 unit[t.value] = 1.0f;
             });
         }
-        float mx = m;
+        float mx = kLowest;
         static_for<0, 2>([&](auto t) {
             float x = s[t.value][0];
             static_for<1, 16>([&](auto i) { x = __builtin_fmaxf(x, s[t.value][i.value]); });
             mx = __builtin_fmaxf(mx, x * unit[t.value]);
         });
-        mx = max_across_32(mx);
+        mx = __builtin_fmaxf(m, M::offset(max_across_32(mx)));
         if (__any(mx > m)) {
             const float shrink = __builtin_amdgcn_exp2f(m - mx);
             m = mx;

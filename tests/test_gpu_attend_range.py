@@ -27,6 +27,54 @@ def _cache(gpu, k, v, page, spare=1):
     return cache, table
 
 
+def _attend64(cache, q, table, length, n, window=None):
+    """(out, lse, what an element may be off) of one sequence.  Of the sum of
+    weighted magnitudes W: the weights' rounding to float16 (2^-11, in
+    bfloat16 2^-9 of the 2^-8 allowed), exponentials and sums in 32 bits (2^-18), scores
+    accumulated in 32 bits (each, and the maximum, within dim * 2^-24 of the
+    sum of magnitudes).  A float16 weight also has a least step, 2^-24 where the
+    largest reach 2^13 at least: half of it is 2^-38 of that one, times codes to
+    448 of its page, whose scale stands for a magnitude of at least 224: 2^-37
+    of the largest magnitude for each key.  Then one rounding of the output."""
+    dtype = {torch.float16: "fp16", torch.bfloat16: "bf16"}[q.dtype]
+    u, d = lm.HALF_ULP[dtype], q.shape[-1]
+    c, x, t = lm.Cache.of(cache), _f64(q), table.cpu().numpy()
+    out, lse, _ = lm.attend(c, x, t, [length], [n], d ** -0.5, window=window, dtype=dtype)
+    sizes = lm.Cache(np.abs(c.k), np.abs(c.v), c.ks, c.vs)
+    weighted, _, _ = lm.attend(lm.Cache(c.k, np.abs(c.v), c.ks, c.vs), x, t, [length], [n], d ** -0.5, window=window, dtype=dtype)
+    k, v = sizes.tokens(t[0], length)
+    size = (np.abs(x) @ k[:, 0].T).max() * d ** -0.5
+    off = weighted * (u + 2.0 ** -18 + 2 * d * 2.0 ** -24 * size)
+    if dtype == "fp16":
+        off += length * 2.0 ** -37 * v.max()
+    return out, lse, off + u * (np.abs(out) + off) + lm.LEAST[dtype]
+
+
+def _check(got, want, bound):
+    off = np.abs(_f64(got) - want)
+    assert (off <= bound).all(), f"worst {np.nanmax(off / bound)} of the bound, {np.isnan(off).sum()} NaN"
+
+
+@pytest.mark.parametrize("length", [180, 3000])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_float16_weights_far_below_the_largest(gpu, dim, heads, n, length):
+    """One key 17.5 above the others' scores, with value 0, and thousands with
+    value 1: their weights are 2^-25.2 of its own, and count."""
+    print("tail", dim, heads, n, length, flush=True)
+    k = torch.zeros(length, 1, dim, device=gpu)
+    k[3, 0, 0] = 10.0
+    v = torch.ones(length, 1, dim, device=gpu)
+    v[3] = 0.0
+    cache, table = _cache(gpu, k, v, 32)
+    q = torch.zeros(n, heads, dim, device=gpu, dtype=torch.float16)
+    q[..., 0] = 1.75 * dim ** 0.5
+    out, lse = attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu), return_lse=True)
+    want, want_lse, bound = _attend64(cache, q, table, length, n)
+    assert bound.max() < 0.05 * want.min()
+    _check(out, want, bound)
+    assert np.abs(_f64(lse) - want_lse).max() <= 2.0 ** -16 * (1 + np.abs(want_lse).max())
+
+
 @pytest.mark.parametrize("length", [150, 3000])
 @pytest.mark.parametrize("sign", [1, -1])
 @pytest.mark.parametrize("dtype,query", [("bf16", 1e33), ("fp16", 6e4)])
