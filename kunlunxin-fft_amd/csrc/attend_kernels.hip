@@ -512,8 +512,10 @@ struct Attend : Item<D> {
     }
 
     // the scales of this lane's sixteen keys, as loaded, and as they count:
-    // scores in units of log 2, NaN for a page number that is none; past the
-    // end of the sequence neither may count, whatever they are
+    // scores in units of log 2, NaN for a page number that is none.  Those of
+    // keys that no row sees may be anything (pages before the window that the
+    // caller has given to others, the stand-in past the end) and must not
+    // count: scores are masked one by one, and values' codes are 0 there.
     float ks_raw, vs_raw;
     bool bad_page;
     __device__ __forceinline__ void load_scales(int entry) {
@@ -523,9 +525,9 @@ struct Attend : Item<D> {
         bad_page = (uint32_t)entry >= (uint32_t)c.pages;
     }
     __device__ __forceinline__ void take_scales(int key0) {
-        const bool in = key0 + 16 * g < seq.len;
+        const int kv = key0 + 16 * g;
         cs = bad_page ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw;
-        vs = in ? vs_raw : 1.0f;
+        vs = kv + 16 > any_lo && kv < any_hi ? vs_raw : 1.0f;
     }
 
     // S = K Q of the group at hand, kw(t, jj) and kx(t) its codes
@@ -936,14 +938,14 @@ struct Tall : Item<D> {
         fvs = c.v_scale[this->page_of(entry) * c.kv_heads + h];
     }
     __device__ __forceinline__ void stash(int buf, int key0) {
+        const int kv = key0 + 16 * wave;
         if (this->block_edge(key0)) {
-            const int kv = key0 + 16 * wave;
             const u32x4 keep = keep_bytes(this->block_lo - kv, this->block_hi - kv);
             static_for<0, L>([&](auto x) { fv[x.value] = this->clean(fv[x.value], keep); });
             if (nan_left) lds.nan = 1;
         }
-        // a page that is none, or the stand-in past the end, may have any scale
-        const float vs = key0 + 16 * wave < seq.len ? fvs : 1.0f;
+        // keys that no row sees may have any scale, see Attend
+        const float vs = kv + 16 > this->block_lo && kv < this->block_hi ? fvs : 1.0f;
         static_for<0, L>([&](auto x) {
             const int i = lane + 64 * x.value;
             if (D % 64 == 0 || i < D) {

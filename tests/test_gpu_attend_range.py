@@ -75,6 +75,32 @@ def test_float16_weights_far_below_the_largest(gpu, dim, heads, n, length):
     assert np.abs(_f64(lse) - want_lse).max() <= 2.0 ** -16 * (1 + np.abs(want_lse).max())
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 2.0 ** 120])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_pages_before_the_window_may_hold_anything(gpu, dim, heads, n, dtype, scale):
+    """Freed pages: entry -1 (which loads read as page 0), or the old number, with
+    NaN codes and any scale.  Sixteen-token pages, so that the first group of
+    keys the rows share has whole ones before the window."""
+    print("window", dim, heads, n, dtype, scale, flush=True)
+    length, page, window = 216 if n == 30 else 200, 16, 30
+    k, v = (_randn((length, 1, dim), "fp32", gpu, s) for s in (310, 311))
+    cache, table = _cache(gpu, k, v, page)
+    q = _randn((n, heads, dim), dtype, gpu, 312)
+    want, _, bound = _attend64(cache, q, table, length, n, window)
+    free = (length - n + 1 - window) // page  # pages no query sees
+    assert free % 4  # the last of them share their group with seen ones
+    old = [0] + table[0, :free].tolist()
+    cache.k.view(torch.uint8)[old] = 0x7f
+    cache.v.view(torch.uint8)[old] = 0x7f
+    cache.k_scale[old] = scale
+    cache.v_scale[old] = scale
+    off, lengths = _i32([0, n], gpu), _i32([length], gpu)
+    _check(attend_paged_cache(cache, q, table, lengths, offsets=off, window=window), want, bound)
+    table[0, :free] = -1
+    _check(attend_paged_cache(cache, q, table, lengths, offsets=off, window=window), want, bound)
+
+
 @pytest.mark.parametrize("length", [150, 3000])
 @pytest.mark.parametrize("sign", [1, -1])
 @pytest.mark.parametrize("dtype,query", [("bf16", 1e33), ("fp16", 6e4)])
