@@ -19,10 +19,13 @@
 // 16-byte load a lane is the matching part of V^T.  m, l and the rescaling of
 // O stay in column j: only the maximum crosses lanes (g), twice per 64 keys.
 //
-// Codes become the queries' type exactly (e4m3 fits both); V's power-of-two
-// scale goes in with the conversion, K's into the 32-bit score.  The weights
-// are rounded to that type for the second product; maxima, sums and O are
-// 32-bit.
+// Codes become the queries' type exactly (e4m3 fits both).  K's power-of-two
+// scale goes into the 32-bit score.  V's goes in with the conversion to
+// bfloat16, which holds every product; float16 does not, and there it goes into
+// the weights, as the exponent it is, and is taken out of l again: 2^(s + e) V
+// with 2^e the scale, m the maximum of s + e, l = sum 2^-e p.  The weights are
+// rounded to the queries' type for the second product, as the matrix
+// instructions need; maxima, sums and O are 32-bit.
 //
 // Bound: for few rows the codes' bytes (one token over 2^18 tokens of 8 heads
 // of 128, 537 MB: 98 us, 5.5 TB/s), for many the products and, not overlapped
@@ -64,8 +67,13 @@ __device__ __forceinline__ float product(float a, float b) {
 // offset gives the same row; m below is the offset.  In float16, whose least
 // step is 2^-24, weights reach 2^13 to 2^14 instead of 1, so that those 2^-25
 // to 2^-38 of the largest, which l counts, are not lost from O.  (A whole
-// number, so that nothing is rounded; past kFusedScores, where 14 would be,
-// the largest score itself.)
+// number, so that nothing is rounded.  Past kFusedScores, where 14 would be, a
+// little less than the largest score, whose weight is then at least 1; kMost
+// holds it in the type.)
+// `shift`: the exponent of a V scale that goes into the weights; `scale` keeps
+// the rest, 1 but for exponents out of [-40, 60].  Below, values are less than
+// 2^-31, nothing in float16; above, more than it holds at any weight that
+// counts.  Between, 2^-e and the weights stay within 32 bits.
 template <class E>
 struct Mat;
 template <>
@@ -83,6 +91,7 @@ struct Mat<__bf16> {
         return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
     }
     static __device__ __forceinline__ float offset(float x) { return x; }
+    static constexpr bool kShifts = false;
 };
 template <>
 struct Mat<_Float16> {
@@ -99,7 +108,14 @@ struct Mat<_Float16> {
         return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI);
     }
     static __device__ __forceinline__ float offset(float x) {
-        return __builtin_fabsf(x) <= kFusedScores ? __builtin_ceilf(x) - 14.0f : x;
+        return __builtin_fabsf(x) <= kFusedScores ? __builtin_ceilf(x) - 14.0f : x * (x > 0.0f ? 1.0f - 0x1p-23f : 1.0f + 0x1p-23f);
+    }
+    static constexpr bool kShifts = true;
+    static constexpr float kMost = 15.0f;
+    static __device__ __forceinline__ int shift(float& scale) {
+        const int e = min(max((int)(__float_as_uint(scale) >> 23) - 127, -40), 60);
+        scale = __builtin_ldexpf(scale, -e);
+        return e;
     }
 };
 
@@ -127,6 +143,15 @@ struct Dims {
     static constexpr int KK = D / 32;        // products of 32 channels
     static constexpr int N = D / 16;         // 16-channel tiles of the output
 };
+
+// a score past kFusedScores less its row's maximum, with what goes in from its
+// page's V scale at most kMost
+template <class M>
+__device__ __forceinline__ float large_score(float s, float unit, float m, int ve) {
+    const float x = product(s, unit) - m;
+    if constexpr (M::kShifts) return x > M::kMost - ve ? M::kMost - ve : x;  // (a NaN stays)
+    else return x;
+}
 
 // a mask of bytes [from, to) of a 16-byte unit
 __device__ __forceinline__ u32x4 keep_bytes(int from, int to) {
@@ -455,6 +480,7 @@ struct Attend : Item<D> {
     u32x2 kx[4];
     u32x4 vw[S::N];
     float cs, vs;
+    int ve = 0;
 
     __device__ __forceinline__ Attend(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
         : I(c_, a_, sh_), lds(lds_) {
@@ -528,6 +554,7 @@ struct Attend : Item<D> {
         const int kv = key0 + 16 * g;
         cs = bad_page ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw;
         vs = kv + 16 > any_lo && kv < any_hi ? vs_raw : 1.0f;
+        if constexpr (M::kShifts) ve = M::shift(vs);
     }
 
     // S = K Q of the group at hand, kw(t, jj) and kx(t) its codes
@@ -568,7 +595,7 @@ struct Attend : Item<D> {
             }
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
-            mx = __builtin_fmaxf(m[r.value], M::offset(max_across_32(max_across_16(mx * unit))));
+            mx = __builtin_fmaxf(m[r.value], M::offset(max_across_32(max_across_16(__builtin_fmaf(mx, unit, (float)ve)))));
             if (__any(mx > m[r.value])) {
                 const float shrink = __builtin_amdgcn_exp2f(m[r.value] - mx);
                 m[r.value] = mx;
@@ -578,22 +605,24 @@ struct Attend : Item<D> {
             }
         });
         float from[R], by = unit;
-        static_for<0, R>([&](auto r) { from[r.value] = -m[r.value]; });
+        static_for<0, R>([&](auto r) { from[r.value] = (float)ve - m[r.value]; });
         if (large) {
             static_for<0, R>([&](auto r) {
                 static_for<0, 16>([&](auto i) {
-                    s[r.value][i.value / 4][i.value % 4] = product(s[r.value][i.value / 4][i.value % 4], unit) - m[r.value];
+                    s[r.value][i.value / 4][i.value % 4] = large_score<M>(s[r.value][i.value / 4][i.value % 4], unit, m[r.value], ve);
                 });
-                from[r.value] = 0.0f;
+                from[r.value] = (float)ve;
             });
             by = 1.0f;
         }
         static_for<0, R>([&](auto r) {
+            float sum = M::kShifts ? 0.0f : l[r.value];
             static_for<0, 16>([&](auto i) {
                 const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r.value][i.value / 4][i.value % 4], by, from[r.value]));
-                l[r.value] += w;
+                sum += w;
                 p[r.value][i.value / 8][i.value % 8] = (E)w;
             });
+            l[r.value] = M::kShifts ? l[r.value] + __builtin_ldexpf(sum, -ve) : sum;
         });
     }
 
@@ -945,7 +974,8 @@ struct Tall : Item<D> {
             if (nan_left) lds.nan = 1;
         }
         // keys that no row sees may have any scale, see Attend
-        const float vs = kv + 16 > this->block_lo && kv < this->block_hi ? fvs : 1.0f;
+        float vs = kv + 16 > this->block_lo && kv < this->block_hi ? fvs : 1.0f;
+        if constexpr (M::kShifts) (void)M::shift(vs);  // the weights' part is weights()'
         static_for<0, L>([&](auto x) {
             const int i = lane + 64 * x.value;
             if (D % 64 == 0 || i < D) {
@@ -961,11 +991,14 @@ struct Tall : Item<D> {
     }
 
     // scales of the keys of this lane's scores, as Attend's load_scales
-    float ks_raw[2], cs[2];
+    float ks_raw[2], cs[2], vs_raw[2];
+    int ve[2] = {0, 0};
     bool bad_page[2];
     __device__ __forceinline__ void load_scales(const int (&entry)[2]) {
         static_for<0, 2>([&](auto t) {
-            ks_raw[t.value] = c.k_scale[this->page_of(entry[t.value]) * c.kv_heads + h];
+            const int64_t at = this->page_of(entry[t.value]) * c.kv_heads + h;
+            ks_raw[t.value] = c.k_scale[at];
+            if constexpr (M::kShifts) vs_raw[t.value] = c.v_scale[at];
             bad_page[t.value] = (uint32_t)entry[t.value] >= (uint32_t)c.pages;
         });
     }
@@ -989,7 +1022,7 @@ struct Tall : Item<D> {
         static_for<0, 2>([&](auto t) {
             float x = s[t.value][0];
             static_for<1, 16>([&](auto i) { x = __builtin_fmaxf(x, s[t.value][i.value]); });
-            mx = __builtin_fmaxf(mx, x * unit[t.value]);
+            mx = __builtin_fmaxf(mx, __builtin_fmaf(x, unit[t.value], (float)ve[t.value]));
         });
         mx = __builtin_fmaxf(m, M::offset(max_across_32(mx)));
         if (__any(mx > m)) {
@@ -999,20 +1032,22 @@ struct Tall : Item<D> {
             l *= shrink;
             static_for<0, D / 32>([&](auto i) { o[i.value] *= shrink; });
         }
-        float from = -m;
+        float from[2] = {(float)ve[0] - m, (float)ve[1] - m};
         if (large) {
             static_for<0, 2>([&](auto t) {
-                static_for<0, 16>([&](auto i) { s[t.value][i.value] = product(s[t.value][i.value], unit[t.value]) - m; });
+                static_for<0, 16>([&](auto i) { s[t.value][i.value] = large_score<M>(s[t.value][i.value], unit[t.value], m, ve[t.value]); });
                 unit[t.value] = 1.0f;
+                from[t.value] = (float)ve[t.value];
             });
-            from = 0.0f;
         }
         static_for<0, 2>([&](auto t) {
+            float sum = M::kShifts ? 0.0f : l;
             static_for<0, 16>([&](auto i) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t.value][i.value], unit[t.value], from));
-                l += w;
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t.value][i.value], unit[t.value], from[t.value]));
+                sum += w;
                 p[2 * t.value + i.value / 8][i.value % 8] = (E)w;
             });
+            l = M::kShifts ? l + __builtin_ldexpf(sum, -ve[t.value]) : sum;
         });
     }
 
@@ -1044,6 +1079,11 @@ struct Tall : Item<D> {
             const bool more = key0 + 64 < end;
             static_for<0, 2>([&](auto t) {
                 cs[t.value] = bad_page[t.value] ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw[t.value];
+                if constexpr (M::kShifts) {
+                    const int kv = key0 + 32 * t.value + 16 * e;
+                    float vs = kv + 16 > this->block_lo && kv < this->block_hi ? vs_raw[t.value] : 1.0f;
+                    ve[t.value] = M::shift(vs);
+                }
             });
             if (more) {
                 load_scales(k1);

@@ -75,6 +75,39 @@ def test_float16_weights_far_below_the_largest(gpu, dim, heads, n, length):
     assert np.abs(_f64(lse) - want_lse).max() <= 2.0 ** -16 * (1 + np.abs(want_lse).max())
 
 
+@pytest.mark.parametrize("length", [180, 3000])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_float16_queries_over_values_of_any_size(gpu, dim, heads, n, length):
+    """Pages of values between 2^-20 and 2^18 in size: no code times its scale
+    may overflow while the mean is finite, and rows before a page of large ones
+    are untouched."""
+    print("values", dim, heads, n, length, flush=True)
+    page = 16
+    k, v = (_randn((length, 1, dim), "fp32", gpu, s) for s in (300, 301))
+    sizes = torch.linspace(-20, 10, -(-length // page), device=gpu).exp2()
+    sizes[-2] = 2.0 ** 16
+    v *= sizes.repeat_interleave(page)[:length, None, None]
+    cache, table = _cache(gpu, k, v, page)
+    assert float(cache.v_scale.max()) >= 2.0 ** 9
+    q = _randn((n, heads, dim), "fp16", gpu, 302, 0.5)
+    out = attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu))
+    want, _, bound = _attend64(cache, q, table, length, n)
+    assert np.abs(want).max() < 60000
+    _check(out, want, bound)
+
+
+def test_float16_values_that_round_up_past_the_type(gpu):
+    """65000 has the code of 65536, which float16 does not hold; their mean with
+    the others it does."""
+    v = torch.full((40, 1, 64), 65000.0, device=gpu)
+    v[::2] = -20000.0
+    cache, table = _cache(gpu, torch.zeros(40, 1, 64, device=gpu), v, 16)
+    q = _randn((40, 2, 64), "fp16", gpu, 303)
+    out = attend_paged_cache(cache, q, table, _i32([40], gpu), offsets=_i32([0, 40], gpu))
+    want, _, bound = _attend64(cache, q, table, 40, 40)
+    _check(out, want, bound)
+
+
 @pytest.mark.parametrize("scale", [float("nan"), float("inf"), 2.0 ** 120])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("dim,heads,n", FORMS)
