@@ -21,7 +21,7 @@ from . import ledger as _ledger
 from . import native
 from .context import device_context, device_ready
 from .rotary import RotaryPlan
-from .runner import current_device, stream_handle
+from .runner import current_device, has_tangent, stream_handle
 
 HEAD_DIMS = (64, 96, 128, 256)
 MAX_PAGE_SIZE = 1024
@@ -123,6 +123,14 @@ def _sequences(cache, page_table, lengths, what, offsets, tokens):
             raise ValueError(f"offsets must have {n + 1} entries, got {offsets.shape[0]}")
 
 
+def _no_gradient(**tensors):
+    grad = torch.is_grad_enabled()
+    for name, t in tensors.items():
+        if t is not None and (grad and t.requires_grad or has_tangent(t)):
+            raise ValueError(f"the cache does not take part in autograd, but {name} does: detach it, or run under "
+                             "torch.no_grad()")
+
+
 def _gpu(cache):
     if not device_ready():
         raise RuntimeError("no ROCm GPU available; cannot run the cache kernels")
@@ -155,7 +163,9 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
     NaN become NaN.  Tokens past the table's width, or whose page number is
     not one of the cache's, are skipped.  No page may belong to two sequences
     of one call.  ``page_table`` ``(sequences, width)``, ``starts`` and
-    ``offsets`` are int32 on the cache's device.
+    ``offsets`` are int32 on the cache's device.  Takes no part in autograd:
+    tensors that require a gradient are refused unless under
+    ``torch.no_grad()``.
     """
     _sequences(cache, page_table, starts, "starts", offsets, None)
     _heads("k", k, cache, heads=cache.kv_heads)
@@ -177,6 +187,7 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
             raise TypeError(f"rotary must be a RotaryPlan, got {type(rotary).__name__}")
         if rotary.head_dim != cache.head_dim:
             raise ValueError(f"the rotary plan is for head_dim {rotary.head_dim}, the cache has {cache.head_dim}")
+    _no_gradient(k=k, v=v, q=q)
     _gpu(cache)
     if q is not None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -209,7 +220,8 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
     sequence is still computed.  ``return_lse``: also the logarithm of the sum
     of exponentials, float32 ``(tokens, q_heads)``, -inf for such a query.
     A sequence longer than its table's pages, or with a page number that is not
-    one of the cache's, gives NaN.
+    one of the cache's, gives NaN.  Takes no part in autograd: a ``q`` that
+    requires a gradient is refused unless under ``torch.no_grad()``.
     """
     _sequences(cache, page_table, lengths, "lengths", offsets, None)
     _heads("q", q, cache)
@@ -225,6 +237,7 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
         raise ValueError(f"window must be None or an int of at least 1, got {window!r}")
     if max_length is not None and (isinstance(max_length, bool) or not isinstance(max_length, int) or max_length < 0):
         raise ValueError(f"max_length must be None or an int of at least 0, got {max_length!r}")
+    _no_gradient(q=q)
     _gpu(cache)
     out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
