@@ -142,35 +142,45 @@ def plan_rotary(head_dim: int, rot_dim: int | None = None, layout: str = "half",
     return RotaryPlan(head_dim, r, layout, tuple(theta), amplitude, max_positions)
 
 
-_torch = None  # the torch module, the dtype ids and the autograd function, once an execute needs them
+# the torch module, the dtype ids, the autograd function and the query for
+# forward-mode tangents, once an execute needs them
+_torch = None
 _DTYPES: dict = {}
 _Rotate = None
+_has_tangent = None
 
 
 def _load_torch():
-    global _torch, _Rotate
+    global _torch, _Rotate, _has_tangent
     import torch
 
-    from . import runner  # noqa: F401  (torch's stream and device queries)
+    from . import runner
 
     native.load()
+
+    def adjacent(t):
+        return t.contiguous() if t.stride(-1) != 1 and t.shape[-1] > 1 else t
 
     class Rotate(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, positions, plan, inverse):
             ctx.save_for_backward(positions)
+            ctx.save_for_forward(positions)
             ctx.plan, ctx.inverse = plan, inverse
             return _launch(plan, x, positions, inverse, None)
 
         @staticmethod
         def backward(ctx, grad):
             # again a Rotate, so that gradients of gradients work
-            if grad.stride(-1) != 1 and grad.shape[-1] > 1:
-                grad = grad.contiguous()
-            return Rotate.apply(grad, ctx.saved_tensors[0], ctx.plan, not ctx.inverse), None, None, None
+            return Rotate.apply(adjacent(grad), ctx.saved_tensors[0], ctx.plan, not ctx.inverse), None, None, None
+
+        @staticmethod
+        def jvp(ctx, tangent, *_):
+            return Rotate.apply(adjacent(tangent), ctx.saved_tensors[0], ctx.plan, ctx.inverse)
 
     _DTYPES.update({torch.float32: native.F32, torch.float16: native.F16, torch.bfloat16: native.BF16})
     _Rotate = Rotate
+    _has_tangent = runner.has_tangent
     _torch = torch
 
 
@@ -230,7 +240,7 @@ def _check(plan, x, positions, out):
             raise TypeError(f"out must be {x.dtype}, got {out.dtype}")
         if out.shape != x.shape or out.stride(-1) != 1:
             raise ValueError(f"out must have x's shape {tuple(x.shape)} and adjacent channels")
-        if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+        if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad) or _has_tangent(x) or _has_tangent(out):
             raise ValueError("out= does not take part in autograd; leave it out, or run under torch.no_grad()")
     if not torch.cuda.is_available():
         raise RuntimeError("no ROCm GPU available; cannot run the rotary kernels")
@@ -246,11 +256,11 @@ def execute_rotary_plan(plan: RotaryPlan, x, positions, *, inverse: bool = False
     ``(batch, tokens)``, int32 or int64) into a new tensor, or into ``out``,
     which may be ``x`` itself.  A position outside ``[0, max_positions)``
     gives NaN.  ``inverse=True`` multiplies by the conjugate roots.  Takes
-    part in autograd."""
+    part in autograd, reverse and forward mode."""
     if _torch is None:
         _load_torch()
     _check(plan, x, positions, out)
     with _ledger.phase("rotary"):
-        if out is None and x.requires_grad and _torch.is_grad_enabled():
+        if out is None and (x.requires_grad and _torch.is_grad_enabled() or _has_tangent(x)):
             return _Rotate.apply(x, positions, plan, bool(inverse))
         return _launch(plan, x, positions, bool(inverse), out)
