@@ -263,4 +263,8 @@ def execute_rotary_plan(plan: RotaryPlan, x, positions, *, inverse: bool = False
     with _ledger.phase("rotary"):
         if out is None and (x.requires_grad and _torch.is_grad_enabled() or _has_tangent(x)):
             return _Rotate.apply(x, positions, plan, bool(inverse))
-        return _launch(plan, x, positions, bool(inverse), out)
+        y = _launch(plan, x, positions, bool(inverse), out)
+        if out is not None and not out.is_inference():
+            # a backward pass that kept `out` must not take the new values for the old
+            _torch.autograd.graph.increment_version(out)
+        return y

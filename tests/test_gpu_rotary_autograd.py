@@ -55,3 +55,29 @@ def test_out_refuses_a_tangent(gpu):
         dual = forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises(ValueError, match="autograd"):
             execute_rotary_plan(plan, dual, torch.arange(8, device=gpu), out=torch.empty_like(x))
+
+
+def test_writing_into_a_saved_tensor_is_noticed(gpu):
+    """A tensor another operation keeps for its backward pass, rotated in place,
+    or written as out: that backward would be wrong, and says so as it does for
+    torch's own in-place operations."""
+    plan = plan_rotary(64)
+    positions = torch.arange(8, device=gpu)
+    for source in ("itself", "another"):
+        x = _x((8, 2, 64), "fp32", gpu, 39)
+        w = _x((64,), "fp32", gpu, 40).requires_grad_()
+        loss = (x * w).sum()
+        execute_rotary_plan(plan, x if source == "itself" else x.clone(), positions, out=x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_out_in_inference_mode(gpu):
+    plan = plan_rotary(64)
+    positions = torch.arange(8, device=gpu)
+    x = _x((8, 2, 64), "fp32", gpu, 41)
+    want = execute_rotary_plan(plan, x, positions)
+    with torch.inference_mode():
+        y = x.clone()
+        assert execute_rotary_plan(plan, y, positions, out=y) is y
+    assert torch.equal(y, want)
