@@ -267,7 +267,8 @@ class NativePlan:
             _RETIRED.append((h, int(self.info.device) if hasattr(self, "info") else 0))
 
 
-# Native plans dropped by their owners, not yet destroyed: (handle, device).
+# Native plans (and rotary plans) dropped by their owners, not yet destroyed:
+# (handle, device).
 # __del__ only appends (atomic under the GIL, and it must not wait on a lock
 # a collection could interrupt); release_retired takes items out under
 # _RETIRED_LOCK, from the front, so two threads releasing at once never
@@ -281,7 +282,7 @@ def retired_count() -> int:
 
 
 def release_retired(sync=None) -> int:
-    """Destroy every retired plan; ``sync(device)`` is called once per
+    """Destroy every retired plan (and rotary plan); ``sync(device)`` is called once per
     device first, to make sure none of their executes is pending.  Returns
     how many plans were destroyed.  Safe to call from several threads."""
     if not _RETIRED or _lib is None:
@@ -295,24 +296,37 @@ def release_retired(sync=None) -> int:
         for dev in sorted({d for _, d in items}):
             sync(dev)
     for h, _ in items:
-        _lib.mfft_plan_destroy(h)
+        if isinstance(h, RotaryHandle):
+            _lib.mfft_rotary_destroy(h)
+        else:
+            _lib.mfft_plan_destroy(h)
     return len(items)
 
 
+class RotaryHandle(ctypes.c_void_p):
+    """``mfft_rotary*``, so that a retired one is known from an ``mfft_plan*``."""
+
+
 class NativeRotary:
-    """Owner of one ``mfft_rotary*`` on the device current at creation.  Its
-    tables are at most a few MB and live as long as the process: the plans
-    that use it are memoised, and freeing it would need every stream done."""
+    """Owner of one ``mfft_rotary*`` on the device current at creation: its
+    tables, of a few hundred KB (2^20 positions of 64 pairs: 1 MB; 2^24 of 256:
+    34 MB).  Retired with the object, as a ``NativePlan``."""
 
     __slots__ = ("handle", "device")
 
     def __init__(self, frequencies, max_positions: int, amplitude: float, layout: str, device: int):
         lib = load()
-        h = ctypes.c_void_p()
+        h = RotaryHandle()
+        self.handle = None
         check(lib.mfft_rotary_create(ctypes.byref(h), (ctypes.c_double * len(frequencies))(*frequencies),
                                      len(frequencies), int(max_positions), float(amplitude), LAYOUT_IDS[layout]))
-        self.handle = h
         self.device = device
+        self.handle = h
+
+    def __del__(self):
+        h, self.handle = getattr(self, "handle", None), None
+        if h is not None and _RETIRED is not None:
+            _RETIRED.append((h, self.device))
 
 
 def rotary_execute(rotary: NativeRotary, args: bytes, stream_ptr: int) -> None:

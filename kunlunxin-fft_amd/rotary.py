@@ -15,6 +15,7 @@ from __future__ import annotations
 import functools
 import math
 import threading
+import weakref
 from dataclasses import dataclass
 
 from . import ledger as _ledger
@@ -64,24 +65,37 @@ class RotaryPlan:
         return self is other
 
     def native(self, device_index: int) -> native.NativeRotary:
-        """This plan's tables on a device (built on first use)."""
-        key = (self, device_index)
+        """This plan's tables on a device (built on first use, kept while the
+        plan is: a HIP graph that uses them needs the plan kept too)."""
+        key = (id(self), device_index)
         hit = _NATIVE.get(key)
-        if hit is None:
-            from .context import device_context
+        if hit is not None and hit[0]() is self:
+            return hit[1]
+        from .context import device_context
+        from .runner import flush_retired_plans
 
-            with _NATIVE_LOCK:
-                hit = _NATIVE.get(key)
-                if hit is None:
-                    with device_context(device_index):
-                        hit = native.NativeRotary(self.frequencies, self.max_positions, self.amplitude, self.layout,
-                                                  device_index)
-                    _NATIVE[key] = hit
-        return hit
+        with _NATIVE_LOCK:
+            hit = _NATIVE.get(key)
+            if hit is None or hit[0]() is not self:
+                flush_retired_plans()
+                with device_context(device_index):
+                    made = native.NativeRotary(self.frequencies, self.max_positions, self.amplitude, self.layout,
+                                               device_index)
+                hit = _NATIVE[key] = (weakref.ref(self, lambda _r: _drop(key, _r)), made)
+        return hit[1]
 
 
+# Tables by plan and device: (weak reference to the plan, tables), dropped when
+# the plan dies (and destroyed later, see native.release_retired).
 _NATIVE: dict = {}
 _NATIVE_LOCK = threading.Lock()
+
+
+def _drop(key, ref) -> None:
+    # not under the lock, which the thread that a collection interrupts may hold
+    hit = _NATIVE.get(key)
+    if hit is not None and hit[0] is ref:
+        _NATIVE.pop(key, None)
 
 
 def _whole(name: str, v) -> int:

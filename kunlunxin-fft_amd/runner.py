@@ -80,6 +80,17 @@ def release_retired_plans() -> int:
     return native.release_retired(_sync_device)
 
 
+def flush_retired_plans() -> None:
+    """Before a native plan is made: destroy the retired ones if many wait.
+    Destroying them synchronises their devices, which would break a graph
+    capture in progress on any thread of the process.  This call can see only
+    its own thread's capture, so it flushes only when it is the process's one
+    Python thread; a multi-threaded caller flushes at points of its choosing
+    (release_retired_plans / clear_native_cache)."""
+    if native.retired_count() >= RETIRED_FLUSH and threading.active_count() == 1:
+        release_retired_plans()
+
+
 def get_native_plan(executed: str, n: int, batch: int, transform_type: str,
                     transform_direction: str, norm: str, block, params: dict,
                     device_index: int) -> native.NativePlan:
@@ -91,13 +102,7 @@ def get_native_plan(executed: str, n: int, batch: int, transform_type: str,
         if p is not None:
             _NATIVE.move_to_end(key)
             return p
-    # Destroying retired plans synchronises their devices, which would break
-    # a graph capture in progress on any thread of the process.  This call
-    # can see only its own thread's capture, so it flushes only when it is
-    # the process's one Python thread; a multi-threaded caller flushes at
-    # points of its choosing (release_retired_plans / clear_native_cache).
-    if native.retired_count() >= RETIRED_FLUSH and threading.active_count() == 1:
-        release_retired_plans()
+    flush_retired_plans()
     with device_context(device_index):
         p = native.NativePlan(n, batch, transform_type, transform_direction, norm, flow, prm,
                               caller_workspace=True)
