@@ -82,7 +82,8 @@ __device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const m
 #pragma unroll
         for (int z = 0; z < V; ++z) {
             const float fa = to_float(half ? f[z] : f[2 * z]), fb = to_float(half ? f[V + z] : f[2 * z + 1]);
-            const E ra = from_float<E>(fa * w[z].x - fb * w[z].y), rb = from_float<E>(fb * w[z].x + fa * w[z].y);
+            const float2 to = rotate_pair({fa, fb}, w[z]);
+            const E ra = from_float<E>(to.x), rb = from_float<E>(to.y);
             if (half) {
                 u.e[z] = ra;
                 v.e[z] = rb;
@@ -252,13 +253,13 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
                 const float2 r = rotary_root(t, p0 + tok, ch * V + x);
                 // pairs (x, V + x), or (2 x, 2 x + 1)
                 const float fa = half ? f[x] : f[2 * x], fb = half ? f[V + x] : f[2 * x + 1];
-                const float ra = fa * r.x - fb * r.y, rb = fb * r.x + fa * r.y;
+                const float2 y = rotate_pair({fa, fb}, r);
                 if (half) {
-                    f[x] = ra;
-                    f[V + x] = rb;
+                    f[x] = y.x;
+                    f[V + x] = y.y;
                 } else {
-                    f[2 * x] = ra;
-                    f[2 * x + 1] = rb;
+                    f[2 * x] = y.x;
+                    f[2 * x + 1] = y.y;
                 }
             }
         };
@@ -346,8 +347,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
         pair_channels(t.layout, t.pairs, e, d0, d1);
         const float fa = to_float(k[i * a.k_strides[0] + d0]), fb = to_float(k[i * a.k_strides[0] + d1]);
         if (e >= t.pairs) return make_float2(fa, fb);
-        const float2 w = rotary_root(t, p0 + i, e);
-        return make_float2(fa * w.x - fb * w.y, fb * w.x + fa * w.y);
+        return rotate_pair({fa, fb}, rotary_root(t, p0 + i, e));
     };
     float mk = 0.0f, mv = 0.0f;
     for (int i = threadIdx.x; i < m * half; i += 256) {

@@ -22,13 +22,22 @@ __device__ __forceinline__ E from_float(float v) {
     return (E)v;  // to nearest, ties to even
 }
 
+// x w as complex values.  Which product is rounded first is written out, as the
+// compiler otherwise chooses for each place: a query turned by the append would
+// differ from one turned alone, and the append turns keys once for their page's
+// scale and, where it cannot hold them, again for their codes, where one unit
+// more in the last place would be past the largest code.
+__device__ __forceinline__ float2 rotate_pair(float2 x, float2 w) {
+    return make_float2(__builtin_fmaf(x.x, w.x, -(x.y * w.y)), __builtin_fmaf(x.y, w.x, x.x * w.y));
+}
+
 // The root of position p, pair j.  p < 0 or past the table: NaN, so that a
 // position the plan does not hold shows in the output.
 __device__ __forceinline__ float2 rotary_root(const RotaryTables& t, int64_t p, int j) {
     if (p < 0 || p >= t.max_positions) return make_float2(__builtin_nanf(""), __builtin_nanf(""));
     const float2 a = t.lo[(p & ((1 << kRotaryLoLog2) - 1)) * t.pairs + j];
     const float2 b = t.hi[(p >> kRotaryLoLog2) * t.pairs + j];
-    return make_float2(a.x * b.x - a.y * b.y, a.x * b.y + a.y * b.x);
+    return rotate_pair(a, b);
 }
 
 // Channels of pair e of a head: the rotated pairs first, then the rest two

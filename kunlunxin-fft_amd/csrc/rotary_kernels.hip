@@ -31,9 +31,9 @@ __global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_r
         const int64_t p = a.positions_64 ? ((const int64_t*)a.positions)[po] : ((const int32_t*)a.positions)[po];
         float2 w = rotary_root(t, p, (int)e);
         if (a.direction == MFFT_INVERSE) w.y = -w.y;
-        const float fa = to_float(va), fb = to_float(vb);
-        va = from_float<E>(fa * w.x - fb * w.y);
-        vb = from_float<E>(fb * w.x + fa * w.y);
+        const float2 z = rotate_pair({to_float(va), to_float(vb)}, w);
+        va = from_float<E>(z.x);
+        vb = from_float<E>(z.y);
     }
     y[d0] = va;
     y[d1] = vb;
@@ -78,9 +78,9 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
         for (int k = 0; k < C; ++k) {
             E& ea = HALF ? u.e[k] : u.e[2 * k];
             E& eb = HALF ? v.e[k] : u.e[2 * k + 1];
-            const float fa = to_float(ea), fb = to_float(eb);
-            ea = from_float<E>(fa * w[k].x - fb * w[k].y);
-            eb = from_float<E>(fb * w[k].x + fa * w[k].y);
+            const float2 z = rotate_pair({to_float(ea), to_float(eb)}, w[k]);
+            ea = from_float<E>(z.x);
+            eb = from_float<E>(z.y);
         }
     };
     int h = h0;
