@@ -39,7 +39,8 @@ def _tensor(name, t, dtype=None):
 
 
 class PagedCache:
-    """The four tensors of a cache, checked once (layout above)."""
+    """The four tensors of a cache, checked once (layout above), and fixed: the
+    kernels use the addresses taken then.  Their contents may be written."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "_packed")
 
@@ -65,11 +66,19 @@ class PagedCache:
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             if tuple(t.shape) != (pages, heads):
                 raise ValueError(f"{name} must have shape {(pages, heads)}, got {tuple(t.shape)}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
-        self.device = k.device
-        self._packed = native.CACHE_ARGS.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                              pages, heads, dim, size)
+        packed = native.CACHE_ARGS.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                        pages, heads, dim, size)
+        for name, value in zip(self.__slots__, (k, v, k_scale, v_scale, pages, heads, size, dim, k.device, packed)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"a PagedCache's {name} cannot be replaced: make another PagedCache of the tensors")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"a PagedCache's {name} cannot be deleted")
+
+    def __reduce__(self):  # a copy takes the addresses of its own tensors
+        return PagedCache, (self.k, self.v, self.k_scale, self.v_scale)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "PagedCache":
