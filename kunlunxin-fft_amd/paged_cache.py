@@ -15,6 +15,8 @@ caller's page table; the library keeps nothing between calls.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import ledger as _ledger
@@ -25,6 +27,8 @@ from .runner import current_device, has_tangent, stream_handle
 
 HEAD_DIMS = (64, 96, 128, 256)
 MAX_PAGE_SIZE = 1024
+# positions of a sequence's table, and of a window
+_MAX_POSITIONS = 1 << 30
 _DTYPES = {torch.float32: native.F32, torch.float16: native.F16, torch.bfloat16: native.BF16}
 # scale of a page nothing was written to: the least there is, so that the
 # first tokens decide
@@ -130,6 +134,22 @@ def _sequences(cache, page_table, lengths, what, offsets, tokens):
         _index("offsets", offsets, cache.device, 1)
         if offsets.shape[0] != n + 1:
             raise ValueError(f"offsets must have {n + 1} entries, got {offsets.shape[0]}")
+
+
+def _scale(value, head_dim) -> float:
+    if value is None:
+        return head_dim ** -0.5
+    try:
+        if isinstance(value, str):
+            raise TypeError
+        scale = float(value)
+    except TypeError:
+        raise TypeError(f"scale must be a number, got {type(value).__name__}") from None
+    except OverflowError:
+        scale = math.inf
+    if not 0.0 <= scale <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scale must be finite in 32 bits and not negative, got {value}")
+    return scale
 
 
 def _no_gradient(**tensors):
@@ -242,10 +262,11 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
     if offsets is None and tokens % lengths.shape[0]:
         raise ValueError(f"without offsets every sequence has as many queries: got {tokens} tokens for "
                          f"{lengths.shape[0]} sequences")
-    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
-        raise ValueError(f"window must be None or an int of at least 1, got {window!r}")
+    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or not 1 <= window <= _MAX_POSITIONS):
+        raise ValueError(f"window must be None or an int in [1, {_MAX_POSITIONS}], got {window!r}")
     if max_length is not None and (isinstance(max_length, bool) or not isinstance(max_length, int) or max_length < 0):
         raise ValueError(f"max_length must be None or an int of at least 0, got {max_length!r}")
+    scale = _scale(scale, cache.head_dim)
     _no_gradient(q=q)
     _gpu(cache)
     out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
@@ -257,8 +278,7 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
             q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1],
             page_table.data_ptr(), lengths.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
             page_table.stride(0), tokens, page_table.shape[1], lengths.shape[0], heads, _DTYPES[q.dtype],
-            cache.head_dim ** -0.5 if scale is None else scale, bool(causal), window or 0,
-            0 if max_length is None else max_length, ws, nbytes)
+            scale, bool(causal), window or 0, 0 if max_length is None else min(max_length, _MAX_POSITIONS), ws, nbytes)
 
     with _ledger.phase("cache-attend"):
         args = pack(0, 0)
