@@ -296,8 +296,10 @@ int mfft_cache_attend(const mfft_cache* c, const mfft_attend_args* a, void* stre
     if (int rc = check_attend(c, a)) return rc;
     if (a->tokens == 0) return MFFT_OK;
     const int64_t D = c->head_dim;
-    if (!a->q || !a->out || !aligned(a->q, 16) || !aligned(a->out, 8) || a->q_strides[0] % 8 || a->q_strides[1] % 8 ||
-        a->out_strides[0] % 4 || a->out_strides[1] % 4)
+    // (the stride of one token, or of one head, is not used)
+    const int64_t n[2] = {a->tokens, a->q_heads};
+    auto keeps = [&](const int64_t* s, int m) { return (n[0] == 1 || s[0] % m == 0) && (n[1] == 1 || s[1] % m == 0); };
+    if (!a->q || !a->out || !aligned(a->q, 16) || !aligned(a->out, 8) || !keeps(a->q_strides, 8) || !keeps(a->out_strides, 4))
         return fail(MFFT_ERR_VALUE, "q must be 16-byte and out 8-byte aligned, with strides that keep it so");
     if (a->lse && !aligned(a->lse, 4)) return fail(MFFT_ERR_VALUE, "lse must be 4-byte aligned");
     if (!distinct({a->tokens, (int64_t)a->q_heads}, a->out_strides, D))
