@@ -392,8 +392,9 @@ typedef struct {
     int64_t k_strides[2], v_strides[2], q_strides[2], q_out_strides[2];  /* token, head; in elements */
     const int32_t* page_table; /* [sequences][table_width] */
     const int32_t* starts;     /* [sequences]: tokens cached before this call */
-    const int32_t* offsets;    /* [sequences + 1]: sequence b's tokens are rows offsets[b] .. offsets[b + 1];
-                                  NULL: one token each */
+    const int32_t* offsets;    /* [sequences + 1], rising: sequence b's tokens are rows offsets[b] ..
+                                  offsets[b + 1]; NULL: one token each.  Other rows are not cached, and
+                                  their q_out is no rotation of theirs */
     int64_t table_stride, tokens;
     int32_t table_width, sequences;
     int32_t q_heads, dtype;
@@ -416,7 +417,8 @@ typedef struct {
     int64_t q_strides[2], out_strides[2];
     const int32_t* page_table;
     const int32_t* lengths;    /* [sequences] */
-    const int32_t* offsets;    /* [sequences + 1], or NULL: tokens / sequences queries each */
+    const int32_t* offsets;    /* [sequences + 1], rising, or NULL: tokens / sequences queries each; rows
+                                  before the first and past the last are no sequence's and see no key */
     int64_t table_stride, tokens;
     int32_t table_width, sequences;
     int32_t q_heads, dtype;    /* MFFT_F16 or MFFT_BF16 */

@@ -1191,6 +1191,26 @@ struct FormOf<E, D, kTall> {
     typedef Tall<E, D> type;
 };
 
+// Rows of no sequence, before the first offset and past the last (padding): they
+// see no key.  Workgroup i of n takes every n-th 256 pieces.  These are
+// workgroups that have nothing else to do, kIdle more than there may be work
+// for: after the work of all workgroups, 0.7 us were added to the shortest call.
+constexpr int kIdle = 32;
+template <class E, int D>
+__device__ __forceinline__ void clear_rest(const mfft_attend_args& a, int64_t i, int64_t n) {
+    if (!a.offsets) return;
+    const int64_t lo = seq_offset(a.offsets, 1, a.tokens, 0), hi = seq_offset(a.offsets, 1, a.tokens, a.sequences);
+    const int64_t pieces = (lo + a.tokens - hi) * a.q_heads * (D / 4);
+    for (i = i * 256 + threadIdx.x; i < pieces; i += n * 256) {
+        const int64_t row = i / (D / 4);
+        const int at = (int)(i % (D / 4)), h = (int)(row % a.q_heads);
+        int64_t tok = row / a.q_heads;
+        if (tok >= lo) tok += hi - lo;
+        *(u32x2*)((E*)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + 4 * at) = u32x2{0, 0};
+        if (a.lse && at == 0) a.lse[tok * a.q_heads + h] = -__builtin_inff();
+    }
+}
+
 template <class E, int D, Form F>
 __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_cache c, mfft_attend_args a, AttendShape sh,
                                                                           float* part_o, float2* part_ml, Cut* cuts) {
@@ -1202,7 +1222,10 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
     int b, item, tile = 0;
     if (sh.grid == 0) {
         b = WorkList{c, a, sh, true, 0, 0}.find(blockIdx.x, before, false);
-        if (b < 0) return;
+        if (b < 0) {
+            clear_rest<E, D>(a, blockIdx.x - before, gridDim.x - before);
+            return;
+        }
         w.seq = sequence(c, a, sh, b);
         item = (int)((int64_t)blockIdx.x - before);
         stop = w.seq.tiles;
@@ -1260,6 +1283,10 @@ __global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_arg
     constexpr int C = (D + 63) / 64;
     const int groups = (sh.live + sh.join_rows - 1) / sh.join_rows;
     const int share = blockIdx.x / groups;
+    if (share >= sh.grid) {
+        clear_rest<E, D>(a, blockIdx.x - sh.grid * groups, gridDim.x - sh.grid * groups);
+        return;
+    }
     const Cut cut = cuts[share];
     if (cut.parts == 0) return;
     const Sequence seq = sequence(c, a, sh, cut.b);
@@ -1315,6 +1342,7 @@ struct AttendLaunch {
     AttendShape sh;
     Form form;
     int64_t grid, o_bytes, ml_bytes, cut_bytes;
+    int idle;  // workgroups more than work, see clear_rest: of the join where there is one
 };
 
 AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a) {
@@ -1341,7 +1369,8 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a) {
     const int64_t longest = a.max_length && a.max_length < table ? a.max_length : table;
     const int64_t each = std::max<int64_t>(1, std::max<int64_t>(a.sequences, a.tokens * w.sh.group / w.sh.rows) * c.kv_heads / at_once);
     const bool whole = longest <= 64 * kWholeTiles * each;
-    w.grid = items;
+    w.idle = a.offsets ? kIdle : 0;
+    w.grid = items + w.idle;
     if (!whole) {
         // as many shares as workgroups run at once
         w.sh.grid = (int)at_once;
@@ -1370,7 +1399,7 @@ void launch_dim(const mfft_cache& c, const mfft_attend_args& a, const AttendLaun
     }
     mark(s);
     if (w.sh.grid) {
-        join_kernel<E, D><<<w.sh.grid * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows), 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+        join_kernel<E, D><<<w.sh.grid * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows) + w.idle, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
         mark(s);
     }
 }

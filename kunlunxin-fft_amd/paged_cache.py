@@ -136,9 +136,7 @@ def _sequences(cache, page_table, lengths, what, offsets, tokens):
             raise ValueError(f"offsets must have {n + 1} entries, got {offsets.shape[0]}")
 
 
-def _scale(value, head_dim) -> float:
-    if value is None:
-        return head_dim ** -0.5
+def _scale(value) -> float:
     try:
         if isinstance(value, str):
             raise TypeError
@@ -152,12 +150,10 @@ def _scale(value, head_dim) -> float:
     return scale
 
 
-def _no_gradient(**tensors):
-    grad = torch.is_grad_enabled()
-    for name, t in tensors.items():
-        if t is not None and (grad and t.requires_grad or has_tangent(t)):
-            raise ValueError(f"the cache does not take part in autograd, but {name} does: detach it, or run under "
-                             "torch.no_grad()")
+def _no_gradient(name, t):
+    if t.requires_grad and torch.is_grad_enabled() or has_tangent(t):
+        raise ValueError(f"the cache does not take part in autograd, but {name} does: detach it, or run under "
+                         "torch.no_grad()")
 
 
 def _gpu(cache):
@@ -181,8 +177,9 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
     float16 or bfloat16, any strides with adjacent channels) to the cache.
 
     Sequence ``b``'s tokens are rows ``offsets[b] .. offsets[b + 1]`` (None:
-    one token a sequence) and take the positions from ``starts[b]`` on, in the
-    pages ``page_table[b]`` names.  With ``rotary`` the keys are rotated by
+    one token a sequence; rows before the first offset and past the last are
+    padding) and take the positions from ``starts[b]`` on, in the pages
+    ``page_table[b]`` names.  With ``rotary`` the keys are rotated by
     their positions first, and ``q`` ``(tokens, q_heads, head_dim)``, if
     given, is rotated in the same launch and returned (without ``rotary``:
     copied).
@@ -216,7 +213,10 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
             raise TypeError(f"rotary must be a RotaryPlan, got {type(rotary).__name__}")
         if rotary.head_dim != cache.head_dim:
             raise ValueError(f"the rotary plan is for head_dim {rotary.head_dim}, the cache has {cache.head_dim}")
-    _no_gradient(k=k, v=v, q=q)
+    _no_gradient("k", k)
+    _no_gradient("v", v)
+    if q is not None:
+        _no_gradient("q", q)
     _gpu(cache)
     if q is not None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -243,7 +243,8 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
     Sequence ``b``'s queries are rows ``offsets[b] .. offsets[b + 1]`` (None:
     as many for every sequence) and are the last of its ``lengths[b]``
     positions.  ``causal``: a query sees the keys up to its own position;
-    ``window``: only that many of the last ones.  A query that sees no key gives 0.
+    ``window``: only that many of the last ones.  A query that sees no key, or
+    is no sequence's (padding before the first offset or past the last), gives 0.
     ``scale`` defaults to ``head_dim ** -0.5``.  ``max_length``, if given,
     bounds ``lengths`` and lets short calls run in one launch; a longer
     sequence is still computed.  ``return_lse``: also the logarithm of the sum
@@ -266,8 +267,8 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
         raise ValueError(f"window must be None or an int in [1, {_MAX_POSITIONS}], got {window!r}")
     if max_length is not None and (isinstance(max_length, bool) or not isinstance(max_length, int) or max_length < 0):
         raise ValueError(f"max_length must be None or an int of at least 0, got {max_length!r}")
-    scale = _scale(scale, cache.head_dim)
-    _no_gradient(q=q)
+    scale = cache.head_dim ** -0.5 if scale is None else _scale(scale)
+    _no_gradient("q", q)
     _gpu(cache)
     out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None

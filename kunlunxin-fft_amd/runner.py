@@ -151,7 +151,12 @@ def current_device() -> int:
 def has_tangent(t) -> bool:
     """Whether ``t`` is a dual tensor of torch's forward-mode differentiation
     (the level is looked at first: unpacking takes half a microsecond)."""
-    return getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(t).tangent is not None
+    try:
+        if _forward_ad._current_level < 0:
+            return False
+    except AttributeError:
+        pass
+    return _forward_ad.unpack_dual(t).tangent is not None
 
 
 def workspace_for(nplan: native.NativePlan, device) -> "torch.Tensor | None":
