@@ -66,14 +66,14 @@ __device__ __forceinline__ float product(float a, float b) {
 // largest score x.  l and O are relative to the same and out = O / l, so any
 // offset gives the same row; m below is the offset.  In float16, whose least
 // step is 2^-24, weights reach 2^13 to 2^14 instead of 1, so that those 2^-25
-// to 2^-38 of the largest, which l counts, are not lost from O.  (A whole
-// number, so that nothing is rounded.  Past kFusedScores, where 14 would be, a
-// little less than the largest score, whose weight is then at least 1; kMost
-// holds it in the type.)
-// `shift`: the exponent of a V scale that goes into the weights; `scale` keeps
-// the rest, 1 but for exponents out of [-40, 60].  Below, values are less than
-// 2^-31, nothing in float16; above, more than it holds at any weight that
-// counts.  Between, 2^-e and the weights stay within 32 bits.
+// to 2^-38 of the largest, which l counts, are not lost from O; the offset
+// moves on once a score is past it by kHead, 14.  (A whole number, so that
+// nothing is rounded.  Past kFusedScores, where 14 would be, a little less than
+// the largest score, whose weight is then at least 1; kMost holds it in the
+// type.)
+// `shift`: the exponent of a V scale that goes into the weights.  Below 2^-40
+// it is taken for that: such values are less than 2^-31, nothing in float16
+// either way, and their 2^-e (a page of zeros has 2^126) stays within 32 bits.
 template <class E>
 struct Mat;
 template <>
@@ -91,6 +91,7 @@ struct Mat<__bf16> {
         return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
     }
     static __device__ __forceinline__ float offset(float x) { return x; }
+    static constexpr float kHead = 0.0f;
     static constexpr bool kShifts = false;
 };
 template <>
@@ -108,15 +109,11 @@ struct Mat<_Float16> {
         return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI);
     }
     static __device__ __forceinline__ float offset(float x) {
-        return __builtin_fabsf(x) <= kFusedScores ? __builtin_ceilf(x) - 14.0f : x * (x > 0.0f ? 1.0f - 0x1p-23f : 1.0f + 0x1p-23f);
+        return __builtin_fabsf(x) <= kFusedScores ? __builtin_ceilf(x) - kHead : x * (x > 0.0f ? 1.0f - 0x1p-23f : 1.0f + 0x1p-23f);
     }
+    static constexpr float kHead = 14.0f, kMost = 15.0f;
     static constexpr bool kShifts = true;
-    static constexpr float kMost = 15.0f;
-    static __device__ __forceinline__ int shift(float& scale) {
-        const int e = min(max((int)(__float_as_uint(scale) >> 23) - 127, -40), 60);
-        scale = __builtin_ldexpf(scale, -e);
-        return e;
-    }
+    static __device__ __forceinline__ int shift(float scale) { return max((int)(__float_as_uint(scale) >> 23) - 127, -40); }
 };
 
 // eight codes times a power-of-two scale
@@ -552,9 +549,14 @@ struct Attend : Item<D> {
     }
     __device__ __forceinline__ void take_scales(int key0) {
         const int kv = key0 + 16 * g;
-        cs = bad_page ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw;
         vs = kv + 16 > any_lo && kv < any_hi ? vs_raw : 1.0f;
-        if constexpr (M::kShifts) ve = M::shift(vs);
+        bool bad = bad_page;
+        if constexpr (M::kShifts) {
+            ve = M::shift(vs);
+            bad |= !(vs < __builtin_inff());
+            vs = 1.0f;
+        }
+        cs = bad ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw;
     }
 
     // S = K Q of the group at hand, kw(t, jj) and kx(t) its codes
@@ -595,8 +597,9 @@ struct Attend : Item<D> {
             }
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
-            mx = __builtin_fmaxf(m[r.value], M::offset(max_across_32(max_across_16(__builtin_fmaf(mx, unit, (float)ve)))));
-            if (__any(mx > m[r.value])) {
+            mx = max_across_32(max_across_16(__builtin_fmaf(mx, unit, (float)ve)));
+            if (__any(mx > m[r.value] + M::kHead)) {
+                mx = __builtin_fmaxf(m[r.value], M::offset(mx));
                 const float shrink = __builtin_amdgcn_exp2f(m[r.value] - mx);
                 m[r.value] = mx;
                 large |= __any(__builtin_fabsf(mx) > kFusedScores && mx > kLowest);
@@ -975,7 +978,7 @@ struct Tall : Item<D> {
         }
         // keys that no row sees may have any scale, see Attend
         float vs = kv + 16 > this->block_lo && kv < this->block_hi ? fvs : 1.0f;
-        if constexpr (M::kShifts) (void)M::shift(vs);  // the weights' part is weights()'
+        if constexpr (M::kShifts) vs = 1.0f;  // it is weights()' there
         static_for<0, L>([&](auto x) {
             const int i = lane + 64 * x.value;
             if (D % 64 == 0 || i < D) {
@@ -1024,8 +1027,9 @@ struct Tall : Item<D> {
             static_for<1, 16>([&](auto i) { x = __builtin_fmaxf(x, s[t.value][i.value]); });
             mx = __builtin_fmaxf(mx, __builtin_fmaf(x, unit[t.value], (float)ve[t.value]));
         });
-        mx = __builtin_fmaxf(m, M::offset(max_across_32(mx)));
-        if (__any(mx > m)) {
+        mx = max_across_32(mx);
+        if (__any(mx > m + M::kHead)) {
+            mx = __builtin_fmaxf(m, M::offset(mx));
             const float shrink = __builtin_amdgcn_exp2f(m - mx);
             m = mx;
             large |= __any(__builtin_fabsf(m) > kFusedScores && m > kLowest);
@@ -1078,12 +1082,14 @@ struct Tall : Item<D> {
             __syncthreads();
             const bool more = key0 + 64 < end;
             static_for<0, 2>([&](auto t) {
-                cs[t.value] = bad_page[t.value] ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw[t.value];
+                bool bad = bad_page[t.value];
                 if constexpr (M::kShifts) {
                     const int kv = key0 + 32 * t.value + 16 * e;
-                    float vs = kv + 16 > this->block_lo && kv < this->block_hi ? vs_raw[t.value] : 1.0f;
+                    const float vs = kv + 16 > this->block_lo && kv < this->block_hi ? vs_raw[t.value] : 1.0f;
                     ve[t.value] = M::shift(vs);
+                    bad |= !(vs < __builtin_inff());
                 }
+                cs[t.value] = bad ? __builtin_nanf("") : a.scale * 1.44269504088896340736f * ks_raw[t.value];
             });
             if (more) {
                 load_scales(k1);

@@ -160,3 +160,18 @@ def test_scores_of_any_size(gpu, dim, heads, n, dtype, query, sign, length):
     u = 2.0 ** -11 if dtype == "fp16" else 0.0
     assert (np.abs(_f64(out) - want) <= (u + lm.HALF_ULP[dtype] + 2.0 ** -20) * np.abs(want) + lm.LEAST[dtype]).all()
     assert (np.abs(_f64(lse) - s[5]) <= 2.0 ** -16 * abs(s[5])).all()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_a_seen_page_whose_scale_is_none_shows(gpu, dim, heads, n, dtype, scale):
+    """Value codes of a page that queries see, under a NaN or infinite scale: NaN
+    in every channel, not a number that looks like a result."""
+    length = 100
+    k, v = (_randn((length, 1, dim), "fp32", gpu, s) for s in (330, 331))
+    cache, table = _cache(gpu, k, v, 16)
+    cache.v_scale[int(table[0, 1])] = scale
+    q = _randn((n, heads, dim), dtype, gpu, 332)
+    out = attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu))
+    assert not torch.isfinite(out).any()

@@ -86,3 +86,16 @@ def test_append_to_many_sequences(gpu, count):
         append_paged_cache(cache, k, v, table, _i32(first, gpu), offsets=_i32(lm.offsets_of(new), gpu))
         want.append(_f64(k), _f64(v), rows, first, new)
         _same(cache, want)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (64, "fp32")])
+def test_append_of_a_padded_batch(gpu, dim, dtype):
+    """Rows before the first offset and past the last are not cached."""
+    counts, starts, before, after = [20, 0, 33], [5, 9, 0], 4, 70
+    table, pool = _table([a + n for a, n in zip(starts, counts)], 16, gpu, 440)
+    cache, own = (PagedCache.empty(pool, 2, dim, 16, gpu) for _ in range(2))
+    off = _i32(lm.offsets_of(counts), gpu)
+    k, v = (_randn((before + 53 + after, 2, dim), dtype, gpu, s) for s in (441, 442))
+    append_paged_cache(cache, k, v, table, _i32(starts, gpu), offsets=off + before)
+    append_paged_cache(own, k[before:before + 53], v[before:before + 53], table, _i32(starts, gpu), offsets=off)
+    _same(cache, lm.Cache.of(own))
