@@ -28,9 +28,9 @@
 // instructions need; maxima, sums and O are 32-bit.
 //
 // Bound: for few rows the codes' bytes (one token over 2^18 tokens of 8 heads
-// of 128, 537 MB: 98 us, 5.5 TB/s), for many the products and, not overlapped
-// with them, the softmax (2048 tokens of 32 heads over 32768: 1.21 ms, 880
-// TFLOP/s; the products alone 732 us).
+// of 128, 537 MB: 99 us, 5.4 TB/s), for many the products and, not overlapped
+// with them, the softmax (2048 tokens of 32 heads over 32768: 1.24 ms, 860
+// TFLOP/s, in float16 1.30 ms; the products alone 732 us).
 #include <algorithm>
 
 #include "lm_device.hpp"
@@ -186,9 +186,15 @@ __device__ __forceinline__ float log_sum(float m, float l, bool poison) {
 // ---- which part of the work a workgroup takes ---------------------------------
 // An item is (sequence, block of query rows, key head); its work is the groups
 // of 64 keys its sequence has.  All items' groups, one item after the other,
-// form one list, and each of `grid` workgroups takes an equal share of it, so
-// that the chip is filled evenly whatever the lengths are: a share is some
-// whole items and at most two cut ones, at its ends.  The list follows from the
+// form one list, and each of `grid` workgroups takes an equal share of it,
+// whatever the lengths are: a share is some whole items and at most two cut
+// ones, at its ends.  (An item is charged all its sequence's groups from the
+// window of the first query on, also those that only later or earlier blocks of
+// rows see, which it leaves out.  Shares of a prompt piece over many cached
+// keys are so within a few percent of equal; those of a prompt of which nothing
+// is cached are not: 8192 tokens of 32 heads 1.16 ms, 475 TFLOP/s, where 2048
+// over 32768 reach 860; nor those of a long piece in a short window: 2048
+// tokens in one of 512, 48 us.)  The list follows from the
 // lengths, which only the device knows; every workgroup works its place out for
 // itself with one pass of a wave over the sequences.  Cut items leave their
 // (m, l, O) in the workspace and join_kernel adds them up.
@@ -223,8 +229,12 @@ constexpr int kCUs = 256;
 constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
 // Up to here, times the items there are for each workgroup at once, an item is
 // never cut: the second launch costs more than it saves, and many items balance
-// by themselves.  One token of one sequence of 1000: 10.7 us whole, 15.1 cut;
-// 256 sequences of up to 1000, mixed: 55 and 111 us.
+// by themselves.  One token a sequence of 32 query and 8 key heads of 128,
+// lengths to the one given (several sequences: mixed), in us, whole and cut:
+// 1 sequence of 1000 10.7 and 15.1, 2000 16.2 and 12.1, 4000 24.8 and 16.2;
+// 8 of 2000 16.2 and 17.0, 4000 26.1 and 19.8, 8000 45 and 34; 256 of 1000 55
+// and 111.  64 of 2000 and 4000, past the bound, would be faster whole: 30 and
+// 54, 55 and 68; of 8000 it is the same, 121.
 constexpr int kWholeTiles = 16;
 
 // the item that starts in share i and is cut at its end: its parts are in
@@ -1360,6 +1370,18 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a) {
     // rows of a sequence and key head, on average where there are offsets
     const int64_t rows = (a.tokens * w.sh.group + a.sequences - 1) / a.sequences;
     const int D = c.head_dim;
+    // 32 sequences of 4096, 8 key heads (4 of dim 256), in us of every form
+    // at 16 / 24 / 32 / 48 / 64 / 96 / 128 rows:
+    //   dim 64   kKeys1 33 35 36 71 59 82 86, kKeys2 39 40 39 46 46 76 79, kKeys4 55 54 53 53 55 97 97,
+    //            kRows 68 67 66 66 66 97 96, kTall 90 89 87 88 87 88 90
+    //   dim 96   kKeys1 43 40 41 100 71 103 117, kKeys2 48 49 49 52 52 107 95, kKeys4 59 60 60 61 63 110 110,
+    //            kRows 77 78 78 78 79 330 328, kTall 114 116 116 117 117 120 124
+    //   dim 128  kKeys1 55 56 57 133 99 137 168, kKeys2 51 51 52 93 94 133 156, kKeys4 75 76 77 78 80 140 143,
+    //            kRows 86 88 86 90 91 138 138, kTall 117 119 117 121 121 125 130
+    //   dim 256  kKeys1 57 91 92 130 165 242 194, kRows 89 91 91 93 96 143 143
+    // and thousands of rows need kTall, which decodes a code once for 128.  What
+    // is taken is not the least everywhere: at 48 and 64 rows kKeys2 would be
+    // at dims to 96, and kKeys4, which is not built for it, at 128.
     w.form = rows <= 16 ? kKeys1 : rows <= 32 && D <= 128 ? kKeys2 : rows <= 64 && D <= 96 ? kKeys4 : rows <= 64 || D > 128 ? kRows : kTall;
     w.sh.rows = w.form == kKeys1 ? 16 : w.form == kKeys2 ? 32 : w.form == kTall ? 128 : 64;
     // a cut costs its rows' partial sums, written and read again: about a

@@ -309,8 +309,7 @@ class RotaryHandle(ctypes.c_void_p):
 
 class NativeRotary:
     """Owner of one ``mfft_rotary*`` on the device current at creation: its
-    tables, of a few hundred KB (2^20 positions of 64 pairs: 1 MB; 2^24 of 256:
-    34 MB).  Retired with the object, as a ``NativePlan``."""
+    tables (2^20 positions of 64 pairs: 1 MB; 2^24 of 256: 36 MB).  Retired with the object, as a ``NativePlan``."""
 
     __slots__ = ("handle", "device")
 

@@ -119,7 +119,7 @@ def _heads(name, t, cache, dtype=None, heads=None):
         raise ValueError(f"{name} must be on {cache.device} like the cache, got {t.device}")
 
 
-def _sequences(cache, page_table, lengths, what, offsets, tokens):
+def _sequences(cache, page_table, lengths, what, offsets):
     if not isinstance(cache, PagedCache):
         raise TypeError(f"cache must be a PagedCache, got {type(cache).__name__}")
     _index("page_table", page_table, cache.device, 2)
@@ -193,7 +193,7 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
     tensors that require a gradient are refused unless under
     ``torch.no_grad()``.
     """
-    _sequences(cache, page_table, starts, "starts", offsets, None)
+    _sequences(cache, page_table, starts, "starts", offsets)
     _heads("k", k, cache, heads=cache.kv_heads)
     _heads("v", v, cache, k.dtype, cache.kv_heads)
     tokens = k.shape[0]
@@ -238,7 +238,9 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
                        return_lse: bool = False):
     """Attention of ``q`` ``(tokens, q_heads, head_dim)`` (float16 or bfloat16;
     ``q_heads`` a multiple of the cache's) over the cache: ``softmax(scale q k)
-    v``, a new tensor of ``q``'s shape and type.
+    v``, a new tensor of ``q``'s shape and type.  Scores, maxima and sums are
+    held in 32 bits; the softmax's weights are rounded to ``q``'s type for the
+    product with ``v``.  ``q`` must be 16-byte aligned, and its strides keep it so.
 
     Sequence ``b``'s queries are rows ``offsets[b] .. offsets[b + 1]`` (None:
     as many for every sequence) and are the last of its ``lengths[b]``
@@ -253,7 +255,7 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
     one of the cache's, gives NaN.  Takes no part in autograd: a ``q`` that
     requires a gradient is refused unless under ``torch.no_grad()``.
     """
-    _sequences(cache, page_table, lengths, "lengths", offsets, None)
+    _sequences(cache, page_table, lengths, "lengths", offsets)
     _heads("q", q, cache)
     if q.dtype is torch.float32:
         raise TypeError("q must be float16 or bfloat16, got torch.float32")
