@@ -28,11 +28,14 @@ def test_plans_that_come_and_go(gpu):
     """A base for every context length: hundreds of plans, each used once."""
     x = torch.randn(3, 1, 32, device=gpu)
     positions = torch.arange(3, device=gpu)
+    plan_rotary.cache_clear()
+    gc.collect()
+    held = len(rotary._NATIVE)  # by others than the cache of plans
     first = execute_rotary_plan(plan_rotary(32, base=5000.0, max_positions=4096), x, positions)
     for i in range(600):
         execute_rotary_plan(plan_rotary(32, base=5000.0 + i, max_positions=4096), x, positions)
     gc.collect()
-    assert len(rotary._NATIVE) <= 256
+    assert len(rotary._NATIVE) <= held + 256
     release_retired_plans()  # a process of one Python thread does so by itself, 64 at a time
     assert native.retired_count() == 0
     assert torch.equal(execute_rotary_plan(plan_rotary(32, base=5000.0, max_positions=4096), x, positions), first)
