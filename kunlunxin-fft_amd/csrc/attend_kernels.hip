@@ -49,11 +49,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr float kLowest = -3.402823466e38f;  // start of the running maximum: no score seen
 
 // Up to here (in units of log 2) a score less its row's maximum is one fma of
-// the unscaled score, whose maximum alone is rounded: off by half a unit of
-// the maximum's last place, 2^-4 at most.  Past it that unit grows until the
-// largest weight is no number; scores are then rounded before the difference,
-// as the maximum is.
-constexpr float kFusedScores = 1048576.0f;
+// the unscaled score, whose maximum alone is rounded: weights are off by half a
+// unit of the maximum's last place, 2^-13.5 of themselves at most (and not all
+// alike: where keys are masked the product is rounded).  That is below what
+// float16 rounds them by, and it grows with the scores until the largest weight
+// is no number; past it the products are rounded before the difference, as the
+// maximum is.
+constexpr float kFusedScores = 4096.0f;
 
 // a b, rounded whatever is done with it
 __device__ __forceinline__ float product(float a, float b) {
@@ -68,9 +70,12 @@ __device__ __forceinline__ float product(float a, float b) {
 // step is 2^-24, weights reach 2^13 to 2^14 instead of 1, so that those 2^-25
 // to 2^-38 of the largest, which l counts, are not lost from O; the offset
 // moves on once a score is past it by kHead, 14.  (A whole number, so that
-// nothing is rounded.  Past kFusedScores, where 14 would be, a little less than
-// the largest score, whose weight is then at least 1; kMost holds it in the
-// type.)
+// nothing is rounded.)
+// `large_offset`: the same past kFusedScores, where s + e below would be rounded
+// and with it what one page's weights are to another's: from the scores alone,
+// by 7 less, or as much less as still can be told from x.  Weights of any values
+// that float16 holds (2^e to 2^8) stay in the type; values past 114688 overflow
+// beside such scores, and those of pages below 2^-22 (2^-15 past 2^24) vanish.
 // `shift`: the exponent of a V scale that goes into the weights.  Below 2^-40
 // it is taken for that: such values are less than 2^-31, nothing in float16
 // either way, and their 2^-e (a page of zeros has 2^126) stays within 32 bits.
@@ -108,10 +113,12 @@ struct Mat<_Float16> {
     static __device__ __forceinline__ x2 decode(uint32_t w, float scale) {
         return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI);
     }
-    static __device__ __forceinline__ float offset(float x) {
-        return __builtin_fabsf(x) <= kFusedScores ? __builtin_ceilf(x) - kHead : x * (x > 0.0f ? 1.0f - 0x1p-23f : 1.0f + 0x1p-23f);
+    static __device__ __forceinline__ float offset(float x) { return __builtin_ceilf(x) - kHead; }
+    static __device__ __forceinline__ float large_offset(float x) {
+        const float y = x - 7.0f;
+        return x - y <= 7.0f ? y : x;
     }
-    static constexpr float kHead = 14.0f, kMost = 15.0f;
+    static constexpr float kHead = 14.0f;
     static constexpr bool kShifts = true;
     static __device__ __forceinline__ int shift(float scale) { return max((int)(__float_as_uint(scale) >> 23) - 127, -40); }
 };
@@ -141,13 +148,19 @@ struct Dims {
     static constexpr int N = D / 16;         // 16-channel tiles of the output
 };
 
-// a score past kFusedScores less its row's maximum, with what goes in from its
-// page's V scale at most kMost
-template <class M>
-__device__ __forceinline__ float large_score(float s, float unit, float m, int ve) {
-    const float x = product(s, unit) - m;
-    if constexpr (M::kShifts) return x > M::kMost - ve ? M::kMost - ve : x;  // (a NaN stays)
-    else return x;
+// A row's offset m, from its largest score (plus e) x and, once `large`, from its
+// largest score alone, which `score` finds.
+template <class M, class S>
+__device__ __forceinline__ float moved_on(float m, float x, bool& large, S&& score) {
+    float to = M::offset(x);
+    large |= __any(__builtin_fabsf(x) > kFusedScores && x > kLowest);
+    if constexpr (M::kShifts) {
+        if (large) {
+            const float y = score();
+            if (__builtin_fabsf(y) > kFusedScores) to = M::large_offset(y);
+        }
+    }
+    return __builtin_fmaxf(m, to);
 }
 
 // a mask of bytes [from, to) of a 16-byte unit
@@ -607,12 +620,11 @@ struct Attend : Item<D> {
             }
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
-            mx = max_across_32(max_across_16(__builtin_fmaf(mx, unit, (float)ve)));
-            if (__any(mx > m[r.value] + M::kHead)) {
-                mx = __builtin_fmaxf(m[r.value], M::offset(mx));
-                const float shrink = __builtin_amdgcn_exp2f(m[r.value] - mx);
-                m[r.value] = mx;
-                large |= __any(__builtin_fabsf(mx) > kFusedScores && mx > kLowest);
+            const float x = max_across_32(max_across_16(__builtin_fmaf(mx, unit, (float)ve)));
+            if ((M::kShifts && large) || __any(x > m[r.value] + M::kHead)) {
+                const float to = moved_on<M>(m[r.value], x, large, [&] { return max_across_32(max_across_16(product(mx, unit))); });
+                const float shrink = __builtin_amdgcn_exp2f(m[r.value] - to);
+                m[r.value] = to;
                 l[r.value] *= shrink;
                 static_for<0, S::N>([&](auto i) { o[r.value][i.value] *= shrink; });
             }
@@ -622,7 +634,7 @@ struct Attend : Item<D> {
         if (large) {
             static_for<0, R>([&](auto r) {
                 static_for<0, 16>([&](auto i) {
-                    s[r.value][i.value / 4][i.value % 4] = large_score<M>(s[r.value][i.value / 4][i.value % 4], unit, m[r.value], ve);
+                    s[r.value][i.value / 4][i.value % 4] = product(s[r.value][i.value / 4][i.value % 4], unit) - m[r.value];
                 });
                 from[r.value] = (float)ve;
             });
@@ -1031,25 +1043,25 @@ struct Tall : Item<D> {
                 unit[t.value] = 1.0f;
             });
         }
-        float mx = kLowest;
+        float mx[2];
         static_for<0, 2>([&](auto t) {
-            float x = s[t.value][0];
-            static_for<1, 16>([&](auto i) { x = __builtin_fmaxf(x, s[t.value][i.value]); });
-            mx = __builtin_fmaxf(mx, __builtin_fmaf(x, unit[t.value], (float)ve[t.value]));
+            mx[t.value] = s[t.value][0];
+            static_for<1, 16>([&](auto i) { mx[t.value] = __builtin_fmaxf(mx[t.value], s[t.value][i.value]); });
         });
-        mx = max_across_32(mx);
-        if (__any(mx > m + M::kHead)) {
-            mx = __builtin_fmaxf(m, M::offset(mx));
-            const float shrink = __builtin_amdgcn_exp2f(m - mx);
-            m = mx;
-            large |= __any(__builtin_fabsf(m) > kFusedScores && m > kLowest);
+        const float x = max_across_32(__builtin_fmaxf(__builtin_fmaf(mx[0], unit[0], (float)ve[0]), __builtin_fmaf(mx[1], unit[1], (float)ve[1])));
+        if ((M::kShifts && large) || __any(x > m + M::kHead)) {
+            const float to = moved_on<M>(m, x, large, [&] {
+                return max_across_32(__builtin_fmaxf(product(mx[0], unit[0]), product(mx[1], unit[1])));
+            });
+            const float shrink = __builtin_amdgcn_exp2f(m - to);
+            m = to;
             l *= shrink;
             static_for<0, D / 32>([&](auto i) { o[i.value] *= shrink; });
         }
         float from[2] = {(float)ve[0] - m, (float)ve[1] - m};
         if (large) {
             static_for<0, 2>([&](auto t) {
-                static_for<0, 16>([&](auto i) { s[t.value][i.value] = large_score<M>(s[t.value][i.value], unit[t.value], m, ve[t.value]); });
+                static_for<0, 16>([&](auto i) { s[t.value][i.value] = product(s[t.value][i.value], unit[t.value]) - m; });
                 unit[t.value] = 1.0f;
                 from[t.value] = (float)ve[t.value];
             });

@@ -175,3 +175,94 @@ def test_a_seen_page_whose_scale_is_none_shows(gpu, dim, heads, n, dtype, scale)
     q = _randn((n, heads, dim), dtype, gpu, 332)
     out = attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu))
     assert not torch.isfinite(out).any()
+
+
+@pytest.mark.parametrize("length", [160, 2048])
+@pytest.mark.parametrize("huge", [-1, 1])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_rows_and_keys_of_very_different_sizes(gpu, dim, heads, n, dtype, huge, length):
+    """The first half of the keys score -2^30 or less: what counts is the second
+    half, as if alone.  And one query head of scores of 2^30 and more beside the
+    others of ordinary ones, which it leaves alone."""
+    print("sizes", dim, heads, n, dtype, huge, length, flush=True)
+    half, page = length // 2, 16
+    k, v = (_randn((length, 1, dim), "fp32", gpu, s) for s in (340, 341))
+    k[:, 0, 0] = 0.25
+    k[:half] = 0.0
+    k[:half, 0, 0] = -1e12 * (1 + torch.arange(half, device=gpu) % 7)
+    cache, table = _cache(gpu, k, v, page)
+    q = _randn((n, heads, dim), dtype, gpu, 342)
+    q[..., 0] = 1.0
+    q[:, 1] *= 1e9 if dtype == "bf16" else 1.0
+    q[:, 1] = torch.where(torch.isfinite(q[:, 1]), q[:, 1], 0.0)
+    if huge < 0:
+        q[:, 1] = 0.0
+        q[:, 1, 0] = -6e4  # the first half's scores are the large ones here, and positive
+    out = _f64(attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu)))
+    others = [h for h in range(heads) if h != 1]
+    want, _, bound = _attend64(cache, q[:, others], table[:, half // page:], half, n)
+    assert (np.abs(out[:, others] - want) <= bound).all()
+    if huge < 0:  # the value of the first keys of the largest score, alone: seven apart, all equal
+        top = lm.Cache.of(cache).tokens(table.cpu().numpy()[0], half)
+        s = top[0][:, 0, 0]
+        want = top[1][s == s.min(), 0].mean(0)
+        size = np.abs(top[1][s == s.min(), 0]).mean(0)
+        assert (np.abs(out[:, 1] - want) <= 2 * lm.HALF_ULP[dtype] * size + 2.0 ** -18 * size + lm.HALF_ULP[dtype] * np.abs(want) + lm.LEAST[dtype]).all()
+    else:
+        assert np.isfinite(out[:, 1]).all()
+
+
+@pytest.mark.parametrize("length", [160, 2048])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_scores_that_grow_from_small_to_huge(gpu, dim, heads, n, dtype, sign, length):
+    """Scores from 2^-20 to 2^36 in the order of the keys, and in the other
+    order: the value of the largest that the row sees, alone."""
+    print("grow", dim, heads, n, dtype, sign, length, flush=True)
+    at = torch.arange(length, device=gpu, dtype=torch.float32)
+    k = torch.zeros(length, 1, dim, device=gpu)
+    # sixteen keys a page share a scale: a power of two each, within what it holds
+    k[:, 0, 0] = torch.exp2(-20 + 56 * torch.floor(at / 16) / (length // 16 - 1)) * (1 + (at % 16) / 16)
+    v = _randn((length, 1, dim), "fp32", gpu, 350)
+    if sign < 0:
+        k, v = k.flip(0), v.flip(0)
+    cache, table = _cache(gpu, k, v, 16)
+    q = torch.zeros(n, heads, dim, device=gpu, dtype=lm.DTYPES[dtype])
+    q[..., 0] = dim ** 0.5
+    out = _f64(attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu)))
+    ks, vs = lm.Cache.of(cache).tokens(table.cpu().numpy()[0], length)
+    for i in range(n):
+        seen = slice(0, length - n + i + 1)
+        s = ks[seen, 0, 0]
+        best = s == s.max()
+        if s.max() < 2.0 ** 10:
+            continue
+        want, size = vs[seen][best, 0].mean(0), np.abs(vs[seen][best, 0]).mean(0)
+        off = (2 * lm.HALF_ULP[dtype] + 2.0 ** -18) * size + lm.HALF_ULP[dtype] * np.abs(want) + lm.LEAST[dtype]
+        assert (np.abs(out[i] - want) <= off).all(), i
+
+
+@pytest.mark.parametrize("exponent", [0, 19, 20, 21, 24, 25, 26, 27, 40, 90])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_equal_scores_of_any_size(gpu, dim, heads, n, dtype, sign, exponent):
+    """Every key scores the same 1.3 * 2^exponent: the mean of the values, whose
+    pages are of sizes from 2^-10 to 2^7 (each scale enters the same)."""
+    print("equal", dim, heads, n, dtype, sign, exponent, flush=True)
+    length, page = 200, 16
+    k = torch.zeros(length, 1, dim, device=gpu)
+    k[..., 0] = 2.0 ** exponent
+    v = _randn((length, 1, dim), "fp32", gpu, 360)
+    v *= torch.linspace(-10, 7, -(-length // page), device=gpu).exp2().repeat_interleave(page)[:length, None, None]
+    cache, table = _cache(gpu, k, v, page)
+    q = torch.zeros(n, heads, dim, device=gpu, dtype=lm.DTYPES[dtype])
+    q[..., 0] = sign * 1.3 * dim ** 0.5
+    out = _f64(attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu)))
+    vs = lm.Cache.of(cache).tokens(table.cpu().numpy()[0], length)[1][:, 0]
+    for i in range(n):
+        want, size = vs[:length - n + i + 1].mean(0), np.abs(vs[:length - n + i + 1]).mean(0)
+        off = (lm.HALF_ULP[dtype] + 2.0 ** -18) * size + lm.HALF_ULP[dtype] * np.abs(want) + lm.LEAST[dtype]
+        assert (np.abs(out[i] - want) <= off).all(), i
