@@ -34,7 +34,7 @@ class RotaryScaling:
       fastest pair alone and divides the slowest by ``factor``;
     * ``"parts"``: pairs that turn at least ``fast`` times over
       ``original_positions`` are left alone, those that turn at most ``slow``
-      times are divided by ``factor``, linearly between.
+      times are divided by ``factor``, linearly in the number of turns between.
 
     ``amplitude`` multiplies the rotated channels.
     """
