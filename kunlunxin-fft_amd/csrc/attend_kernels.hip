@@ -67,10 +67,11 @@ __device__ __forceinline__ float product(float a, float b) {
 // `offset`: what a row's weights are relative to, 2^(s - offset), from its
 // largest score x.  l and O are relative to the same and out = O / l, so any
 // offset gives the same row; m below is the offset.  In float16, whose least
-// step is 2^-24, weights reach 2^13 to 2^14 instead of 1, so that those 2^-25
-// to 2^-38 of the largest, which l counts, are not lost from O; the offset
-// moves on once a score is past it by kHead, 14.  (A whole number, so that
-// nothing is rounded.)
+// step is 2^-24, the largest weight is 2^14 instead of 1, so that those 2^-25
+// to 2^-38 of it, which l counts, are not lost from O; the offset is the largest
+// score less 14, and moves on once a score is past it by kMost, 15.  (A power of
+// two, so that the type's rounding leaves a weight without others alone: a row
+// that sees one key gives its value.)
 // `large_offset`: the same past kFusedScores, where s + e below would be rounded
 // and with it what one page's weights are to another's: from the scores alone,
 // by 7 less, or as much less as still can be told from x.  Weights of any values
@@ -96,7 +97,7 @@ struct Mat<__bf16> {
         return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
     }
     static __device__ __forceinline__ float offset(float x) { return x; }
-    static constexpr float kHead = 0.0f;
+    static constexpr float kMost = 0.0f;
     static constexpr bool kShifts = false;
 };
 template <>
@@ -113,12 +114,12 @@ struct Mat<_Float16> {
     static __device__ __forceinline__ x2 decode(uint32_t w, float scale) {
         return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI);
     }
-    static __device__ __forceinline__ float offset(float x) { return __builtin_ceilf(x) - kHead; }
+    static __device__ __forceinline__ float offset(float x) { return x - 14.0f; }
     static __device__ __forceinline__ float large_offset(float x) {
         const float y = x - 7.0f;
         return x - y <= 7.0f ? y : x;
     }
-    static constexpr float kHead = 14.0f;
+    static constexpr float kMost = 15.0f;
     static constexpr bool kShifts = true;
     static __device__ __forceinline__ int shift(float scale) { return max((int)(__float_as_uint(scale) >> 23) - 127, -40); }
 };
@@ -621,7 +622,7 @@ struct Attend : Item<D> {
             float mx = s[r.value][0][0];
             static_for<1, 16>([&](auto i) { mx = __builtin_fmaxf(mx, s[r.value][i.value / 4][i.value % 4]); });
             const float x = max_across_32(max_across_16(__builtin_fmaf(mx, unit, (float)ve)));
-            if ((M::kShifts && large) || __any(x > m[r.value] + M::kHead)) {
+            if ((M::kShifts && large) || __any(x > m[r.value] + M::kMost)) {
                 const float to = moved_on<M>(m[r.value], x, large, [&] { return max_across_32(max_across_16(product(mx, unit))); });
                 const float shrink = __builtin_amdgcn_exp2f(m[r.value] - to);
                 m[r.value] = to;
@@ -1049,7 +1050,7 @@ struct Tall : Item<D> {
             static_for<1, 16>([&](auto i) { mx[t.value] = __builtin_fmaxf(mx[t.value], s[t.value][i.value]); });
         });
         const float x = max_across_32(__builtin_fmaxf(__builtin_fmaf(mx[0], unit[0], (float)ve[0]), __builtin_fmaf(mx[1], unit[1], (float)ve[1])));
-        if ((M::kShifts && large) || __any(x > m + M::kHead)) {
+        if ((M::kShifts && large) || __any(x > m + M::kMost)) {
             const float to = moved_on<M>(m, x, large, [&] {
                 return max_across_32(__builtin_fmaxf(product(mx[0], unit[0]), product(mx[1], unit[1])));
             });

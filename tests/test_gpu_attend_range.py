@@ -266,3 +266,22 @@ def test_equal_scores_of_any_size(gpu, dim, heads, n, dtype, sign, exponent):
         want, size = vs[:length - n + i + 1].mean(0), np.abs(vs[:length - n + i + 1]).mean(0)
         off = (lm.HALF_ULP[dtype] + 2.0 ** -18) * size + lm.HALF_ULP[dtype] * np.abs(want) + lm.LEAST[dtype]
         assert (np.abs(out[i] - want) <= off).all(), i
+
+
+@pytest.mark.parametrize("size", [0.01, 1.0, 40.0, 3000.0])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,n", FORMS)
+def test_a_single_key_gives_its_value(gpu, dim, heads, n, dtype, size):
+    """With a window of one, and for a sequence of one key: the value itself, not
+    nearly (a weight of one is a power of two, rounded by nothing)."""
+    print("single", dim, heads, n, dtype, size, flush=True)
+    length, page = 100, 16
+    k, v = (_randn((length, 1, dim), "fp32", gpu, s) for s in (370, 371))
+    v *= torch.linspace(-6, 6, -(-length // page), device=gpu).exp2().repeat_interleave(page)[:length, None, None]
+    cache, table = _cache(gpu, k, v, page)
+    q = _randn((n, heads, dim), dtype, gpu, 372, size)
+    vs = lm.Cache.of(cache).tokens(table.cpu().numpy()[0], length)[1]
+    out = _f64(attend_paged_cache(cache, q, table, _i32([length], gpu), offsets=_i32([0, n], gpu), window=1))
+    np.testing.assert_array_equal(out, np.broadcast_to(vs[length - n:], out.shape))
+    out = _f64(attend_paged_cache(cache, q[:1], table, _i32([1], gpu), offsets=_i32([0, 1], gpu)))
+    np.testing.assert_array_equal(out, np.broadcast_to(vs[:1], out.shape))
