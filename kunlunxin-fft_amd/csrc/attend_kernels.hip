@@ -29,8 +29,8 @@
 //
 // Bound: for few rows the codes' bytes (one token over 2^18 tokens of 8 heads
 // of 128, 537 MB: 99 us, 5.4 TB/s), for many the products and, not overlapped
-// with them, the softmax (2048 tokens of 32 heads over 32768: 1.24 ms, 860
-// TFLOP/s, in float16 1.30 ms; the products alone 732 us).
+// with them, the softmax (2048 tokens of 32 heads over 32768: 1.23 ms, 870
+// TFLOP/s, in float16 1.31 ms; the products alone 732 us).
 #include <algorithm>
 
 #include "lm_device.hpp"
