@@ -357,6 +357,17 @@ typedef struct {
 } mfft_rotary_args;
 int mfft_rotary_execute(const mfft_rotary* rotary, const mfft_rotary_args* args, void* stream);
 
+/* Positions with several axes (time, height, width): pair j is turned by axis
+ * axis_of[j] (0 <= axis_of[j] < axes <= MFFT_MAX_AXES) of its token's
+ * position, each axis' positions below max_positions.  mfft_rotary_execute
+ * refuses such a plan (of two axes or more); mfft_rotary_execute_axes reads
+ * axis a's positions axis_stride * a elements after args->positions, and takes
+ * plans of one axis too. */
+enum { MFFT_MAX_AXES = 4 };
+int mfft_rotary_create_axes(mfft_rotary** out, const double* frequencies, const int32_t* axis_of, int32_t pairs,
+                            int32_t axes, int64_t max_positions, double amplitude, int layout);
+int mfft_rotary_execute_axes(const mfft_rotary* rotary, const mfft_rotary_args* args, int64_t axis_stride, void* stream);
+
 /* A paged cache.  Codes are e4m3 (1 sign, 4 exponent, 3 fraction bits, bias 7,
  * largest 448, one NaN, no infinities); a page's value is code * scale, the
  * scale a power of two, the least one with every magnitude at most 448 * scale.
@@ -400,6 +411,30 @@ typedef struct {
     int32_t q_heads, dtype;
 } mfft_append_args;
 int mfft_cache_append(const mfft_cache* cache, const mfft_rotary* rotary, const mfft_append_args* args, void* stream);
+/* As mfft_cache_append with a rotary, but row n is turned by the positions at
+ * positions[axis_stride * a + token_stride * n] of the rotary's axes a (int32,
+ * or int64 with positions_64), whatever its place in the cache.  A position
+ * out of the rotary's range gives NaN. */
+int mfft_cache_append_at(const mfft_cache* cache, const mfft_rotary* rotary, const mfft_append_args* args,
+                         const void* positions, int64_t axis_stride, int64_t token_stride, int32_t positions_64,
+                         void* stream);
+
+/* Cached tokens read back: rows offsets[b] .. offsets[b + 1] of k and v are
+ * code * scale of positions starts[b], starts[b] + 1, ... of sequence b,
+ * rounded to the type.  A position below 0 or past the table's width, and a
+ * page number that is none, give NaN; rows of no sequence 0. */
+typedef struct {
+    void* k;                   /* [tokens][kv_heads][head_dim] */
+    void* v;
+    int64_t k_strides[2], v_strides[2];  /* token, head; in elements */
+    const int32_t* page_table; /* [sequences][table_width] */
+    const int32_t* starts;     /* [sequences] */
+    const int32_t* offsets;    /* [sequences + 1], rising, or NULL: tokens / sequences rows each */
+    int64_t table_stride, tokens;
+    int32_t table_width, sequences;
+    int32_t dtype;             /* MFFT_F32 / F16 / BF16 */
+} mfft_read_args;
+int mfft_cache_read(const mfft_cache* cache, const mfft_read_args* args, void* stream);
 
 /* Attention of q [tokens][q_heads][head_dim] over the cache: q_heads a
  * multiple of kv_heads, query head h reads key head h / (q_heads / kv_heads).

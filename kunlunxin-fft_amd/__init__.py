@@ -13,7 +13,7 @@ module name ``kunlunxin_fft_amd`` (``__graft_entry__.load_package()`` or
 Beside the transforms stand the operators a language model's step needs next
 to them: rotary positions (``plan_rotary``, ``execute_rotary_plan``) and a
 paged 8-bit key and value cache with its attention (``PagedCache``,
-``append_paged_cache``, ``attend_paged_cache``).
+``append_paged_cache``, ``attend_paged_cache``, ``read_paged_cache``).
 
 Host-only names (planning, tables, configs) import without torch;
 torch-dependent names (runners) resolve lazily on first access, as in the
@@ -47,7 +47,7 @@ from .entry import (  # noqa: F401
 )
 from .composition import composition_select, load_composition_table  # noqa: F401
 from .error_metric import max_rel_error, rel_l2  # noqa: F401
-from .rotary import RotaryPlan, RotaryScaling, execute_rotary_plan, plan_rotary  # noqa: F401
+from .rotary import RotaryAxes, RotaryPlan, RotaryScaling, execute_rotary_plan, plan_rotary  # noqa: F401
 from .selector import Selection, assert_current_environment, load_table, select  # noqa: F401
 
 _TORCH_ATTRS = {
@@ -77,6 +77,7 @@ _TORCH_ATTRS = {
     "PagedCache": "paged_cache",
     "append_paged_cache": "paged_cache",
     "attend_paged_cache": "paged_cache",
+    "read_paged_cache": "paged_cache",
     "log2_exact": "validate",
     "time_call": "runner",
     "time_call_detailed": "runner",
@@ -88,7 +89,7 @@ _TORCH_ATTRS = {
 
 __all__ = [
     "ConfigError", "DesignSpace", "DeviceProfile", "ExecutionPlan",
-    "ExecutionReport", "Manifest", "RotaryPlan", "RotaryScaling", "Selection", "SizeMatrix", "SUPPORTED_NORMS", "SUPPORTED_TRANSFORMS",
+    "ExecutionReport", "Manifest", "RotaryAxes", "RotaryPlan", "RotaryScaling", "Selection", "SizeMatrix", "SUPPORTED_NORMS", "SUPPORTED_TRANSFORMS",
     "SUPPORTED_TRANSFORM_DIRECTIONS", "assert_current_environment", "build_manifest",
     "composition_select", "execute_fft_plan", "execute_rotary_plan", "git_commit", "git_dirty",
     "load_composition_table", "load_table", "max_rel_error", "norm_scale", "plan_fft", "plan_rotary", "rel_l2",

@@ -51,8 +51,9 @@ __host__ __device__ inline AppendGrid append_grid(const mfft_cache& c, const mff
 }
 
 // Queries: thread i takes V pairs of a token and `grid.q_heads` of its heads.
-template <class E, int V>
-__device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const AppendGrid& grid, int64_t at) {
+template <class E, int V, bool PLACED>
+__device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& places,
+                             const AppendGrid& grid, int64_t at) {
     struct alignas(V * sizeof(E)) Vec {
         E e[V];
     };
@@ -63,14 +64,19 @@ __device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const m
     const int64_t n = ts / (uint32_t)grid.q_slabs;
     if (n >= a.tokens) return;
     const int h0 = (int)(ts % (uint32_t)grid.q_slabs) * grid.q_heads, h1 = min(h0 + grid.q_heads, a.q_heads);
-    const int b = token_sequence(a.offsets, 1, a.tokens, a.sequences, n);
-    const int64_t p = a.starts[b] + (n - seq_offset(a.offsets, 1, a.tokens, b));
+    int64_t p = 0;
+    if constexpr (!PLACED) {
+        const int b = token_sequence(a.offsets, 1, a.tokens, a.sequences, n);
+        p = a.starts[b] + (n - seq_offset(a.offsets, 1, a.tokens, b));
+    }
     const bool turned = ch * V < t.pairs, half = t.layout == MFFT_ROTARY_HALF;
     const int d0 = turned && half ? ch * V : ch * 2 * V, d1 = turned && half ? d0 + t.pairs : d0 + V;
     float2 w[V];
     if (turned)
 #pragma unroll
-        for (int x = 0; x < V; ++x) w[x] = rotary_root(t, p, ch * V + x);
+        for (int x = 0; x < V; ++x)
+            w[x] = PLACED ? axis_root(t, places.p, places.wide, n * places.token_stride, places.axis_stride, ch * V + x)
+                          : rotary_root(t, p, ch * V + x);
     const E* x = (const E*)a.q + n * a.q_strides[0] + h0 * a.q_strides[1];
     E* y = (E*)a.q_out + n * a.q_out_strides[0] + h0 * a.q_out_strides[1];
     auto turn = [&](Vec& u, Vec& v) {
@@ -139,12 +145,13 @@ __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d)
     return r;
 }
 
-template <class E, bool WIDE>
-__global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache c, mfft_append_args a) {
+// PLACED: tokens are turned by positions of their own, not by their places.
+template <class E, bool WIDE, bool PLACED>
+__global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache c, mfft_append_args a, Positions places) {
     constexpr int W = WIDE ? 16 / (int)sizeof(E) : 1;
     const AppendGrid grid = append_grid(c, a, W);
     if ((int64_t)blockIdx.x >= grid.kv_blocks) {
-        rotate_query<E, W>(t, c, a, grid, ((int64_t)blockIdx.x - grid.kv_blocks) * 256 + threadIdx.x);
+        rotate_query<E, W, PLACED>(t, c, a, places, grid, ((int64_t)blockIdx.x - grid.kv_blocks) * 256 + threadIdx.x);
         return;
     }
     const int64_t slot = blockIdx.x / c.kv_heads;
@@ -178,6 +185,11 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
     const int m = (int)(p1 - p0);       // tokens written
     const int64_t row = row0 + (p0 - start);
 
+    // root of pair e of the i-th of these tokens
+    auto root = [&](int i, int e) {
+        if constexpr (PLACED) return axis_root(t, places.p, places.wide, (row + i) * places.token_stride, places.axis_stride, e);
+        else return rotary_root(t, p0 + i, e);
+    };
     const E* k = (const E*)a.k + row * a.k_strides[0] + h * a.k_strides[1];
     const E* v = (const E*)a.v + row * a.v_strides[0] + h * a.v_strides[1];
     uint8_t* kc = (uint8_t*)c.k + (page * c.kv_heads + h) * (int64_t)P * D;
@@ -252,7 +264,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
             const bool half = t.layout == MFFT_ROTARY_HALF;
 #pragma unroll
             for (int x = 0; x < V; ++x) {
-                const float2 r = rotary_root(t, p0 + tok, ch * V + x);
+                const float2 r = root(tok, ch * V + x);
                 // pairs (x, V + x), or (2 x, 2 x + 1)
                 const float fa = half ? f[x] : f[2 * x], fb = half ? f[V + x] : f[2 * x + 1];
                 const float2 y = rotate_pair({fa, fb}, r);
@@ -349,7 +361,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
         pair_channels(t.layout, t.pairs, e, d0, d1);
         const float fa = to_float(k[i * a.k_strides[0] + d0]), fb = to_float(k[i * a.k_strides[0] + d1]);
         if (e >= t.pairs) return make_float2(fa, fb);
-        return rotate_pair({fa, fb}, rotary_root(t, p0 + i, e));
+        return rotate_pair({fa, fb}, root(i, e));
     };
     float mk = 0.0f, mv = 0.0f;
     for (int i = threadIdx.x; i < m * half; i += 256) {
@@ -391,15 +403,21 @@ bool wide(const RotaryTables& t, const mfft_append_args& a) {
     return true;
 }
 
-template <class E>
-void launch_type(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, hipStream_t s) {
+template <class E, bool PLACED>
+void launch_form(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& at, hipStream_t s) {
     if (wide(t, a)) {
         const AppendGrid g = append_grid(c, a, a.dtype == MFFT_F32 ? 4 : 8);
-        append_kernel<E, true><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a);
+        append_kernel<E, true, PLACED><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a, at);
     } else {
         const AppendGrid g = append_grid(c, a, 1);
-        append_kernel<E, false><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a);
+        append_kernel<E, false, PLACED><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a, at);
     }
+}
+
+template <class E>
+void launch_type(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& at, hipStream_t s) {
+    if (at.p) launch_form<E, true>(t, c, a, at, s);
+    else launch_form<E, false>(t, c, a, at, s);
 }
 
 }  // namespace
@@ -409,10 +427,11 @@ bool append_launch_fits(const RotaryTables&, const mfft_cache& c, const mfft_app
     return launch_fits(g.kv_blocks + g.q_blocks, 256);
 }
 
-hipError_t launch_append(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, hipStream_t stream) {
-    if (a.dtype == MFFT_F32) launch_type<float>(t, c, a, stream);
-    else if (a.dtype == MFFT_F16) launch_type<_Float16>(t, c, a, stream);
-    else launch_type<__bf16>(t, c, a, stream);
+hipError_t launch_append(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& at,
+                         hipStream_t stream) {
+    if (a.dtype == MFFT_F32) launch_type<float>(t, c, a, at, stream);
+    else if (a.dtype == MFFT_F16) launch_type<_Float16>(t, c, a, at, stream);
+    else launch_type<__bf16>(t, c, a, at, stream);
     mark(stream);
     return hipGetLastError();
 }

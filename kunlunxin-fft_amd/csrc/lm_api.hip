@@ -116,8 +116,9 @@ int check_device(const mfft_rotary* r) {
 
 extern "C" {
 
-int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pairs, int64_t max_positions,
-                       double amplitude, int layout) {
+// axis_of: NULL with one axis
+static int create_rotary(mfft_rotary** out, const double* frequencies, const int32_t* axis_of, int32_t pairs, int32_t axes,
+                         int64_t max_positions, double amplitude, int layout) {
     mfft::clear_error();
     if (!out) return fail(MFFT_ERR_VALUE, "out must not be NULL");
     *out = nullptr;
@@ -131,6 +132,9 @@ int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pai
     for (int j = 0; j < pairs; ++j)
         if (!std::isfinite(frequencies[j]) || std::fabs(frequencies[j]) > 1e3)
             return fail(MFFT_ERR_VALUE, "frequency %d must be finite and at most 1000 radians a position", j);
+    for (int j = 0; axis_of && j < pairs; ++j)
+        if (axis_of[j] < 0 || axis_of[j] >= axes)
+            return fail(MFFT_ERR_VALUE, "axis_of[%d] must be in [0, %d), got %d", j, axes, axis_of[j]);
     mfft_rotary* r = nullptr;
     try {
         r = new mfft_rotary();
@@ -147,6 +151,8 @@ int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pai
         };
         const std::vector<float2> lo = rows(lo_rows < max_positions ? lo_rows : max_positions, 1, 1.0L);
         const std::vector<float2> hi = rows(hi_rows, lo_rows, (long double)amplitude);
+        std::vector<float2> axis(axes > 1 ? (pairs + 7) / 8 : 0);
+        for (int j = 0; axes > 1 && j < pairs; ++j) ((uint8_t*)axis.data())[j] = (uint8_t)axis_of[j];
         hipStream_t us = nullptr;
         int rc = MFFT_OK;
         hipError_t e = hipGetDevice(&r->device);
@@ -154,6 +160,7 @@ int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pai
         if (rc == MFFT_OK) rc = mfft::upload_stream(r->device, &us);
         if (rc == MFFT_OK) rc = mfft::upload(&r->lo, lo, &r->table_bytes, us);
         if (rc == MFFT_OK) rc = mfft::upload(&r->hi, hi, &r->table_bytes, us);
+        if (rc == MFFT_OK && axes > 1) rc = mfft::upload(&r->axis, axis, &r->table_bytes, us);
         if (us) {
             e = hipStreamSynchronize(us);  // also after a failure: the host tables die here
             if (e != hipSuccess && rc == MFFT_OK) rc = hip_fail(e, "hipStreamSynchronize(rotary tables)");
@@ -162,7 +169,7 @@ int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pai
             mfft_rotary_destroy(r);
             return rc;
         }
-        r->t = {r->lo, r->hi, max_positions, pairs, layout};
+        r->t = {r->lo, r->hi, max_positions, pairs, layout, axes, (const uint8_t*)r->axis};
         *out = r;
         return MFFT_OK;
     } catch (const std::bad_alloc&) {
@@ -174,17 +181,30 @@ int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pai
     }
 }
 
+int mfft_rotary_create(mfft_rotary** out, const double* frequencies, int32_t pairs, int64_t max_positions,
+                       double amplitude, int layout) {
+    return create_rotary(out, frequencies, nullptr, pairs, 1, max_positions, amplitude, layout);
+}
+
+int mfft_rotary_create_axes(mfft_rotary** out, const double* frequencies, const int32_t* axis_of, int32_t pairs,
+                            int32_t axes, int64_t max_positions, double amplitude, int layout) {
+    mfft::clear_error();
+    if (out) *out = nullptr;
+    if (axes < 1 || axes > MFFT_MAX_AXES) return fail(MFFT_ERR_VALUE, "axes must be in [1, %d], got %d", MFFT_MAX_AXES, axes);
+    if (!axis_of) return fail(MFFT_ERR_VALUE, "axis_of must not be NULL");
+    return create_rotary(out, frequencies, axis_of, pairs, axes, max_positions, amplitude, layout);
+}
+
 int mfft_rotary_destroy(mfft_rotary* r) {
     if (!r) return MFFT_OK;
+    if (r->axis) (void)hipFree(r->axis);
     if (r->lo) (void)hipFree(r->lo);
     if (r->hi) (void)hipFree(r->hi);
     delete r;
     return MFFT_OK;
 }
 
-int mfft_rotary_execute(const mfft_rotary* r, const mfft_rotary_args* a, void* stream) {
-    mfft::clear_error();
-    if (!r || !a) return fail(MFFT_ERR_VALUE, "rotary and args must not be NULL");
+static int execute_rotary(const mfft_rotary* r, const mfft_rotary_args* a, int64_t axis_stride, void* stream) {
     if (int rc = check_dtype(a->dtype, true)) return rc;
     if (a->direction != MFFT_FORWARD && a->direction != MFFT_INVERSE)
         return fail(MFFT_ERR_VALUE, "unsupported direction %d", a->direction);
@@ -212,12 +232,25 @@ int mfft_rotary_execute(const mfft_rotary* r, const mfft_rotary_args* a, void* s
     if (!mfft::rotary_launch_fits(r->t, *a))
         return fail(MFFT_ERR_UNSUPPORTED, "batch=%lld of %lld tokens needs a launch of 2^32 work-items or more; split it",
                     (long long)a->batch, (long long)a->tokens);
-    const hipError_t e = mfft::launch_rotary(r->t, *a, (hipStream_t)stream);
+    const hipError_t e = mfft::launch_rotary(r->t, *a, axis_stride, (hipStream_t)stream);
     return e == hipSuccess ? MFFT_OK : hip_fail(e, "kernel launch");
 }
 
-int mfft_cache_append(const mfft_cache* c, const mfft_rotary* r, const mfft_append_args* a, void* stream) {
+int mfft_rotary_execute(const mfft_rotary* r, const mfft_rotary_args* a, void* stream) {
     mfft::clear_error();
+    if (!r || !a) return fail(MFFT_ERR_VALUE, "rotary and args must not be NULL");
+    if (r->t.axes > 1) return fail(MFFT_ERR_VALUE, "the rotary takes positions of %d axes: mfft_rotary_execute_axes", r->t.axes);
+    return execute_rotary(r, a, 0, stream);
+}
+
+int mfft_rotary_execute_axes(const mfft_rotary* r, const mfft_rotary_args* a, int64_t axis_stride, void* stream) {
+    mfft::clear_error();
+    if (!r || !a) return fail(MFFT_ERR_VALUE, "rotary and args must not be NULL");
+    if (int rc = check_strides("positions", {(int64_t)r->t.axes}, &axis_stride)) return rc;
+    return execute_rotary(r, a, axis_stride, stream);
+}
+
+static int append(const mfft_cache* c, const mfft_rotary* r, const mfft_append_args* a, const mfft::Positions& at, void* stream) {
     if (int rc = check_cache(c)) return rc;
     if (!a) return fail(MFFT_ERR_VALUE, "args must not be NULL");
     if (int rc = check_dtype(a->dtype, true)) return rc;
@@ -253,7 +286,62 @@ int mfft_cache_append(const mfft_cache* c, const mfft_rotary* r, const mfft_appe
     }
     if (!mfft::append_launch_fits(r ? r->t : mfft::RotaryTables{}, *c, *a))
         return fail(MFFT_ERR_UNSUPPORTED, "%lld tokens need a launch of 2^32 work-items or more; split the call", (long long)a->tokens);
-    const hipError_t e = mfft::launch_append(r ? r->t : mfft::RotaryTables{}, *c, *a, (hipStream_t)stream);
+    const hipError_t e = mfft::launch_append(r ? r->t : mfft::RotaryTables{}, *c, *a, at, (hipStream_t)stream);
+    return e == hipSuccess ? MFFT_OK : hip_fail(e, "kernel launch");
+}
+
+int mfft_cache_append(const mfft_cache* c, const mfft_rotary* r, const mfft_append_args* a, void* stream) {
+    mfft::clear_error();
+    if (r && r->t.axes > 1)
+        return fail(MFFT_ERR_VALUE, "the rotary takes positions of %d axes: mfft_cache_append_at", r->t.axes);
+    return append(c, r, a, mfft::Positions{}, stream);
+}
+
+int mfft_cache_append_at(const mfft_cache* c, const mfft_rotary* r, const mfft_append_args* a, const void* positions,
+                         int64_t axis_stride, int64_t token_stride, int32_t positions_64, void* stream) {
+    mfft::clear_error();
+    if (!r || !a) return fail(MFFT_ERR_VALUE, "rotary and args must not be NULL");
+    if (int rc = check_strides("positions", {(int64_t)r->t.axes}, &axis_stride)) return rc;
+    if (a->tokens > 0) {
+        if (int rc = check_strides("positions", {a->tokens}, &token_stride)) return rc;
+        if (!positions || !aligned(positions, positions_64 ? 8 : 4))
+            return fail(MFFT_ERR_VALUE, "positions must not be NULL and be aligned to their elements");
+    }
+    return append(c, r, a, mfft::Positions{positions, axis_stride, token_stride, positions_64}, stream);
+}
+
+int mfft_cache_read(const mfft_cache* c, const mfft_read_args* a, void* stream) {
+    mfft::clear_error();
+    if (int rc = check_cache(c)) return rc;
+    if (!a) return fail(MFFT_ERR_VALUE, "args must not be NULL");
+    if (int rc = check_dtype(a->dtype, true)) return rc;
+    if (int rc = check_sequences(a->tokens, a->sequences, a->table_width, a->table_stride, a->page_table, a->starts, "starts"))
+        return rc;
+    if (a->offsets && !aligned(a->offsets, 4)) return fail(MFFT_ERR_VALUE, "offsets must be 4-byte aligned");
+    if (!a->offsets && a->tokens % a->sequences)
+        return fail(MFFT_ERR_VALUE, "without offsets every sequence has as many rows: %lld tokens, %d sequences",
+                    (long long)a->tokens, a->sequences);
+    if (int rc = check_strides("k", {a->tokens, (int64_t)c->kv_heads}, a->k_strides)) return rc;
+    if (int rc = check_strides("v", {a->tokens, (int64_t)c->kv_heads}, a->v_strides)) return rc;
+    if (int rc = check_device(nullptr)) return rc;
+    if (a->tokens == 0) return MFFT_OK;
+    const int es = dtype_size(a->dtype);
+    if (!a->k || !a->v || !aligned(a->k, es) || !aligned(a->v, es))
+        return fail(MFFT_ERR_VALUE, "k and v must not be NULL and be aligned to their elements");
+    if (!distinct({a->tokens, (int64_t)c->kv_heads}, a->k_strides, c->head_dim) ||
+        !distinct({a->tokens, (int64_t)c->kv_heads}, a->v_strides, c->head_dim))
+        return fail(MFFT_ERR_VALUE, "k's or v's strides make its elements overlap");
+    const Extent ek = extent(a->k, {a->tokens, (int64_t)c->kv_heads}, a->k_strides, c->head_dim, es);
+    const Extent ev = extent(a->v, {a->tokens, (int64_t)c->kv_heads}, a->v_strides, c->head_dim, es);
+    if (overlap(ek, ev)) return fail(MFFT_ERR_VALUE, "k and v must not overlap");
+    const int64_t codes = c->pages * c->kv_heads * (int64_t)c->page_size * c->head_dim;
+    for (const Extent& e : {ek, ev})
+        for (const void* p : {c->k, c->v})
+            if (overlap(e, Extent{(const char*)p, (const char*)p + codes}))
+                return fail(MFFT_ERR_VALUE, "k and v must not overlap the cache");
+    if (!mfft::read_launch_fits(*c, *a))
+        return fail(MFFT_ERR_UNSUPPORTED, "%lld tokens need a launch of 2^32 work-items or more; split the call", (long long)a->tokens);
+    const hipError_t e = mfft::launch_read(*c, *a, (hipStream_t)stream);
     return e == hipSuccess ? MFFT_OK : hip_fail(e, "kernel launch");
 }
 

@@ -40,6 +40,18 @@ __device__ __forceinline__ float2 rotary_root(const RotaryTables& t, int64_t p, 
     return rotate_pair(a, b);
 }
 
+__device__ __forceinline__ int64_t position(const void* p, int32_t wide, int64_t at) {
+    return wide ? ((const int64_t*)p)[at] : ((const int32_t*)p)[at];
+}
+
+// The root of pair j of the token whose positions stand from p[at] on, with
+// several axes.
+__device__ __forceinline__ float2 axis_root(const RotaryTables& t, const void* p, int32_t wide, int64_t at,
+                                            int64_t axis_stride, int j) {
+    const int x = t.axes > 1 ? t.axis[j] : 0;
+    return rotary_root(t, position(p, wide, at + x * axis_stride), j);
+}
+
 // Channels of pair e of a head: the rotated pairs first, then the rest two
 // by two.
 __device__ __forceinline__ void pair_channels(int layout, int pairs, int e, int& d0, int& d1) {

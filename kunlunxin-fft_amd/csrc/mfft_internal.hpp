@@ -171,7 +171,7 @@ hipError_t launch_fourstep(int dir, const float2* src, float2* dst, char* fws, c
 hipError_t launch_fourstep_real(const float2* src, float2* dst, float2* work, const mfft_plan* p, float scale,
                                 hipStream_t stream);
 
-// ---- rotary_kernels.hip, append_kernels.hip, attend_kernels.hip ------------
+// ---- rotary_kernels.hip, append_kernels.hip, read_kernels.hip, attend_kernels.hip
 // Roots m exp(i p theta_j) of a position p are the product of a row of `lo`
 // (p mod 1024) and one of `hi` (p / 1024): see mfft_rotary below.
 constexpr int kRotaryLoLog2 = 10;
@@ -181,11 +181,24 @@ struct RotaryTables {
     int64_t max_positions;  // 0: no rotation
     int32_t pairs;
     int32_t layout;
+    int32_t axes;           // of a position; 0 and 1: one
+    const uint8_t* axis;    // [pairs], with several axes: the one that turns each pair
 };
-hipError_t launch_rotary(const RotaryTables& t, const mfft_rotary_args& a, hipStream_t stream);
+// Positions that do not follow from a token's place: axis x of token n at
+// p[x * axis_stride + n * token_stride].
+struct Positions {
+    const void* p;          // NULL: they do
+    int64_t axis_stride, token_stride;
+    int32_t wide;           // int64, else int32
+};
+// (the token strides are the arguments')
+hipError_t launch_rotary(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_stride, hipStream_t stream);
 bool rotary_launch_fits(const RotaryTables& t, const mfft_rotary_args& a);
-hipError_t launch_append(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, hipStream_t stream);
+hipError_t launch_append(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& at,
+                         hipStream_t stream);
 bool append_launch_fits(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a);
+hipError_t launch_read(const mfft_cache& c, const mfft_read_args& a, hipStream_t stream);
+bool read_launch_fits(const mfft_cache& c, const mfft_read_args& a);
 bool attend_supported(int head_dim);
 bool attend_launch_fits(const mfft_cache& c, const mfft_attend_args& a);
 int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a);
@@ -202,5 +215,6 @@ struct mfft_rotary {
     mfft::RotaryTables t{};
     float2* lo = nullptr;
     float2* hi = nullptr;
+    float2* axis = nullptr;  // bytes: the axis of each pair
     int64_t table_bytes = 0;
 };

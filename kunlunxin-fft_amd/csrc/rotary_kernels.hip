@@ -13,9 +13,9 @@ namespace mfft {
 namespace {
 
 // One thread per (token, head, pair), any strides, alignment and sizes.
-template <class E>
-__global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_rotary_args a, uint32_t half_dim,
-                                                          uint32_t total) {
+template <class E, bool AXES>
+__global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_rotary_args a, int64_t axis_stride,
+                                                          uint32_t half_dim, uint32_t total) {
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     if (i >= total) return;
     const uint32_t e = i % half_dim, th = i / half_dim;
@@ -28,8 +28,8 @@ __global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_r
     E* y = (E*)a.out + b * a.out_strides[0] + n * a.out_strides[1] + h * a.out_strides[2];
     E va = x[d0], vb = x[d1];
     if ((int)e < t.pairs) {
-        const int64_t p = a.positions_64 ? ((const int64_t*)a.positions)[po] : ((const int32_t*)a.positions)[po];
-        float2 w = rotary_root(t, p, (int)e);
+        float2 w = AXES ? axis_root(t, a.positions, a.positions_64, po, axis_stride, (int)e)
+                        : rotary_root(t, position(a.positions, a.positions_64, po), (int)e);
         if (a.direction == MFFT_INVERSE) w.y = -w.y;
         const float2 z = rotate_pair({to_float(va), to_float(vb)}, w);
         va = from_float<E>(z.x);
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
     float2 w[C];
     if (turned) {
         const int64_t po = b * a.position_strides[0] + n * a.position_strides[1];
-        const int64_t p = a.positions_64 ? ((const int64_t*)a.positions)[po] : ((const int32_t*)a.positions)[po];
+        const int64_t p = position(a.positions, a.positions_64, po);
 #pragma unroll
         for (int x = 0; x < C; ++x) {
             w[x] = rotary_root(t, p, (int)c * C + x);
@@ -131,8 +131,8 @@ int heads_a_thread(int64_t threads, int heads) {
 }
 
 template <class E>
-void launch_type(const RotaryTables& t, const mfft_rotary_args& a, hipStream_t s) {
-    if (chunked(t, a)) {
+void launch_type(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_stride, hipStream_t s) {
+    if (t.axes <= 1 && chunked(t, a)) {
         const bool half = t.layout == MFFT_ROTARY_HALF;
         const uint32_t chunks = (uint32_t)(a.head_dim * sizeof(E) / (half ? 32 : 16));
         const uint32_t total = (uint32_t)(a.batch * a.tokens) * chunks;
@@ -144,7 +144,9 @@ void launch_type(const RotaryTables& t, const mfft_rotary_args& a, hipStream_t s
     }
     const uint32_t half = (uint32_t)a.head_dim / 2;
     const uint32_t total = (uint32_t)(a.batch * a.tokens * a.heads) * half;
-    rotary_pair_kernel<E><<<(uint32_t)(((uint64_t)total + 255) / 256), 256, 0, s>>>(t, a, half, total);
+    const uint32_t grid = (uint32_t)(((uint64_t)total + 255) / 256);
+    if (t.axes > 1) rotary_pair_kernel<E, true><<<grid, 256, 0, s>>>(t, a, axis_stride, half, total);
+    else rotary_pair_kernel<E, false><<<grid, 256, 0, s>>>(t, a, 0, half, total);
 }
 
 }  // namespace
@@ -154,10 +156,10 @@ bool rotary_launch_fits(const RotaryTables&, const mfft_rotary_args& a) {
     return a.batch <= (kMaxLaunchItems - 256) / a.heads / half / a.tokens;
 }
 
-hipError_t launch_rotary(const RotaryTables& t, const mfft_rotary_args& a, hipStream_t stream) {
-    if (a.dtype == MFFT_F32) launch_type<float>(t, a, stream);
-    else if (a.dtype == MFFT_F16) launch_type<_Float16>(t, a, stream);
-    else launch_type<__bf16>(t, a, stream);
+hipError_t launch_rotary(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_stride, hipStream_t stream) {
+    if (a.dtype == MFFT_F32) launch_type<float>(t, a, axis_stride, stream);
+    else if (a.dtype == MFFT_F16) launch_type<_Float16>(t, a, axis_stride, stream);
+    else launch_type<__bf16>(t, a, axis_stride, stream);
     mark(stream);
     return hipGetLastError();
 }

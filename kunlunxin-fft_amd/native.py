@@ -43,7 +43,9 @@ EXPORTS = (
     "mfft_execute_ws", "mfft_execute_noalloc", "mfft_twiddle_transpose", "mfft_stream_copy",
     "mfft_r2c_stitch", "mfft_c2r_pre", "mfft_c2r_unpack",
     "mfft_rotary_create", "mfft_rotary_destroy", "mfft_rotary_execute",
-    "mfft_cache_append", "mfft_cache_attend_workspace", "mfft_cache_attend",
+    "mfft_rotary_create_axes", "mfft_rotary_execute_axes",
+    "mfft_cache_append", "mfft_cache_append_at", "mfft_cache_read",
+    "mfft_cache_attend_workspace", "mfft_cache_attend",
 )
 PLAN_CALLER_WORKSPACE = 1
 
@@ -56,6 +58,8 @@ ROTARY_ARGS = struct.Struct("@3P10q5i4x")
 CACHE_ARGS = struct.Struct("@4Pq3i4x")
 APPEND_ARGS = struct.Struct("@4P8q3P2q4i")
 ATTEND_ARGS = struct.Struct("@3P4q3P2q4ifi2qPq")
+READ_ARGS = struct.Struct("@2P4q3P2q3i4x")
+MAX_AXES = 4
 
 
 class PlanInfo(ctypes.Structure):
@@ -149,6 +153,16 @@ def load() -> ctypes.CDLL:
         lib.mfft_rotary_destroy.restype = i32
         lib.mfft_rotary_execute.argtypes = [vp, ctypes.c_char_p, vp]
         lib.mfft_rotary_execute.restype = i32
+        lib.mfft_rotary_create_axes.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_double),
+                                                ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.c_int32, i64,
+                                                ctypes.c_double, i32]
+        lib.mfft_rotary_create_axes.restype = i32
+        lib.mfft_rotary_execute_axes.argtypes = [vp, ctypes.c_char_p, i64, vp]
+        lib.mfft_rotary_execute_axes.restype = i32
+        lib.mfft_cache_append_at.argtypes = [ctypes.c_char_p, vp, ctypes.c_char_p, vp, i64, i64, ctypes.c_int32, vp]
+        lib.mfft_cache_append_at.restype = i32
+        lib.mfft_cache_read.argtypes = [ctypes.c_char_p, ctypes.c_char_p, vp]
+        lib.mfft_cache_read.restype = i32
         lib.mfft_cache_append.argtypes = [ctypes.c_char_p, vp, ctypes.c_char_p, vp]
         lib.mfft_cache_append.restype = i32
         lib.mfft_cache_attend_workspace.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(i64)]
@@ -313,12 +327,18 @@ class NativeRotary:
 
     __slots__ = ("handle", "device")
 
-    def __init__(self, frequencies, max_positions: int, amplitude: float, layout: str, device: int):
+    def __init__(self, frequencies, max_positions: int, amplitude: float, layout: str, device: int, axis_of=()):
         lib = load()
         h = RotaryHandle()
         self.handle = None
-        check(lib.mfft_rotary_create(ctypes.byref(h), (ctypes.c_double * len(frequencies))(*frequencies),
-                                     len(frequencies), int(max_positions), float(amplitude), LAYOUT_IDS[layout]))
+        n = len(frequencies)
+        theta = (ctypes.c_double * n)(*frequencies)
+        if axis_of:
+            check(lib.mfft_rotary_create_axes(ctypes.byref(h), theta, (ctypes.c_int32 * n)(*axis_of), n,
+                                              max(axis_of) + 1, int(max_positions), float(amplitude), LAYOUT_IDS[layout]))
+        else:
+            check(lib.mfft_rotary_create(ctypes.byref(h), theta, n, int(max_positions), float(amplitude),
+                                         LAYOUT_IDS[layout]))
         self.device = device
         self.handle = h
 
@@ -330,6 +350,26 @@ class NativeRotary:
 
 def rotary_execute(rotary: NativeRotary, args: bytes, stream_ptr: int) -> None:
     rc = _lib.mfft_rotary_execute(rotary.handle, args, stream_ptr)
+    if rc:
+        check(rc)
+
+
+def rotary_execute_axes(rotary: NativeRotary, args: bytes, axis_stride: int, stream_ptr: int) -> None:
+    rc = _lib.mfft_rotary_execute_axes(rotary.handle, args, axis_stride, stream_ptr)
+    if rc:
+        check(rc)
+
+
+def cache_append_at(cache: bytes, rotary: NativeRotary, args: bytes, positions_ptr: int, axis_stride: int,
+                    token_stride: int, positions_64: bool, stream_ptr: int) -> None:
+    rc = load().mfft_cache_append_at(cache, rotary.handle, args, positions_ptr, axis_stride, token_stride, positions_64,
+                                     stream_ptr)
+    if rc:
+        check(rc)
+
+
+def cache_read(cache: bytes, args: bytes, stream_ptr: int) -> None:
+    rc = load().mfft_cache_read(cache, args, stream_ptr)
     if rc:
         check(rc)
 

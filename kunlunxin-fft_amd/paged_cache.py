@@ -1,5 +1,5 @@
-"""A paged 8-bit cache of keys and values, the append that fills it and the
-attention that reads it.
+"""A paged 8-bit cache of keys and values, the append that fills it, the
+attention that reads it, and its tokens read back.
 
 Codes are e4m3; each page and head shares a power-of-two scale for its keys
 and one for its values, the least with every magnitude at most 448 of it:
@@ -171,8 +171,26 @@ def _on_device(device, fn, *args):
         return fn(*args, stream_handle(dev))
 
 
+def _positions(rotary, positions, tokens, cache):
+    """Checks what tokens are turned by, where that is not their place."""
+    if positions is None:
+        if rotary is not None and rotary.axes:
+            raise ValueError(f"the rotary plan takes positions of {rotary.axes} axes: give positions")
+        return
+    if rotary is None:
+        raise ValueError("positions are what the rotary plan turns by: give rotary")
+    _tensor("positions", positions)
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    want = (rotary.axes, tokens) if rotary.axes else (tokens,)
+    if tuple(positions.shape) != want:
+        raise ValueError(f"positions must have shape {want}, got {tuple(positions.shape)}")
+    if positions.device != cache.device:
+        raise ValueError(f"positions must be on {cache.device} like the cache, got {positions.device}")
+
+
 def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=None, rotary: RotaryPlan | None = None,
-                       q=None):
+                       q=None, positions=None):
     """Write new keys and values ``(tokens, kv_heads, head_dim)`` (float32,
     float16 or bfloat16, any strides with adjacent channels) to the cache.
 
@@ -182,7 +200,10 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
     ``page_table[b]`` names.  With ``rotary`` the keys are rotated by
     their positions first, and ``q`` ``(tokens, q_heads, head_dim)``, if
     given, is rotated in the same launch and returned (without ``rotary``:
-    copied).
+    copied).  ``positions`` ``(tokens,)`` (int32 or int64; ``(axes, tokens)``
+    for a plan with axes, which needs them) are what tokens are rotated by
+    instead of their places in the cache; one that the plan does not hold
+    gives NaN.
 
     A token in a page's first slot opens the page anew.  A page whose later
     tokens need a larger scale has its codes rescaled.  Infinities and
@@ -213,6 +234,7 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
             raise TypeError(f"rotary must be a RotaryPlan, got {type(rotary).__name__}")
         if rotary.head_dim != cache.head_dim:
             raise ValueError(f"the rotary plan is for head_dim {rotary.head_dim}, the cache has {cache.head_dim}")
+    _positions(rotary, positions, tokens, cache)
     _no_gradient("k", k)
     _no_gradient("v", v)
     if q is not None:
@@ -228,9 +250,49 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
         0 if offsets is None else offsets.data_ptr(), page_table.stride(0), tokens, page_table.shape[1],
         starts.shape[0], heads, _DTYPES[k.dtype])
     with _ledger.phase("cache-append"):
-        _on_device(cache.device, native.cache_append, cache._packed,
-                   None if rotary is None else rotary.native(k.get_device()), args)
+        table = None if rotary is None else rotary.native(k.get_device())
+        if positions is None:
+            _on_device(cache.device, native.cache_append, cache._packed, table, args)
+        else:
+            ps = positions.stride()
+            _on_device(cache.device, native.cache_append_at, cache._packed, table, args, positions.data_ptr(),
+                       ps[0] if rotary.axes else 0, ps[-1], positions.dtype is torch.int64)
     return out
+
+
+def read_paged_cache(cache: PagedCache, page_table, starts, tokens: int, *, offsets=None, dtype=torch.bfloat16):
+    """The keys and values of cached tokens, two new tensors ``(tokens,
+    kv_heads, head_dim)`` of ``dtype`` (float32, float16 or bfloat16): codes
+    times their page's scale, exact in float32 and bfloat16, rounded (and
+    infinite past its range) in float16.
+
+    The inverse of ``append_paged_cache``: rows ``offsets[b] .. offsets[b + 1]``
+    (None: as many for every sequence) are sequence ``b``'s tokens from
+    position ``starts[b]`` on, in the pages ``page_table[b]`` names; keys are
+    as they were cached, rotated.  Rows before the first offset and past the
+    last are 0.  A position below 0 or past the table's width, and a page number
+    that is not one of the cache's, give NaN.  ``page_table`` ``(sequences,
+    width)``, ``starts`` and ``offsets`` are int32 on the cache's device.
+    """
+    _sequences(cache, page_table, starts, "starts", offsets)
+    if isinstance(tokens, bool) or not isinstance(tokens, int):
+        raise TypeError(f"tokens must be an int, got {type(tokens).__name__}")
+    if not 0 <= tokens < 1 << 31:
+        raise ValueError(f"tokens must be in [0, 2^31), got {tokens}")
+    if offsets is None and tokens % starts.shape[0]:
+        raise ValueError(f"without offsets every sequence has as many tokens: got {tokens} for {starts.shape[0]} sequences")
+    if dtype not in _DTYPES:
+        raise TypeError(f"dtype must be torch.float32, torch.float16 or torch.bfloat16, got {dtype}")
+    _gpu(cache)
+    k, v = (torch.empty((tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device) for _ in range(2))
+    s = k.stride()
+    args = native.READ_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), s[0], s[1], s[0], s[1], page_table.data_ptr(), starts.data_ptr(),
+        0 if offsets is None else offsets.data_ptr(), page_table.stride(0), tokens, page_table.shape[1],
+        starts.shape[0], _DTYPES[dtype])
+    with _ledger.phase("cache-read"):
+        _on_device(cache.device, native.cache_read, cache._packed, args)
+    return k, v
 
 
 def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=None, scale: float | None = None,

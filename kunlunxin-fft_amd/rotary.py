@@ -7,6 +7,9 @@ from two tables made in extended precision on the host.  Channels past
 ``rot_dim`` are copied.  The gradient is the product with the conjugate roots
 (``inverse=True``), which autograd takes by itself.
 
+With several axes (``RotaryAxes``: time, height, width of a picture's or a
+film's patches) each pair is turned by one axis of its token's position.
+
 ``plan_rotary`` is host-only, as ``plan_fft`` is; the tables go to a device
 with the first execute there.
 """
@@ -48,6 +51,28 @@ class RotaryScaling:
 
 
 @dataclass(frozen=True)
+class RotaryAxes:
+    """Positions with several axes: axis ``a`` turns ``pairs[a]`` of the pairs.
+
+    * ``order``: ``"blocks"``, axis 0's pairs first, then axis 1's; or
+      ``"cycle"``, one pair of each axis in turn, axes that have all of theirs
+      left out;
+    * ``ladder``: ``"shared"``, pair ``j`` has the frequency it has with one
+      axis, ``base^(-2 j / rot_dim)``; or ``"own"``, the ``i``-th pair of an
+      axis has ``base^(-i / pairs[a])``, as if the axis had a head of its own.
+    """
+
+    pairs: tuple
+    order: str = "blocks"
+    ladder: str = "shared"
+
+    def __post_init__(self):
+        # here, as (8.0, 24.0) would find the plan memoised for (8, 24)
+        if not isinstance(self.pairs, tuple) or not all(type(n) is int for n in self.pairs):
+            raise TypeError(f"pairs must be a tuple of ints, got {self.pairs!r}")
+
+
+@dataclass(frozen=True)
 class RotaryPlan:
     """A resolved rotation; made by ``plan_rotary``, reused over calls."""
 
@@ -57,6 +82,8 @@ class RotaryPlan:
     frequencies: tuple
     amplitude: float
     max_positions: int
+    axis_of: tuple = ()  # the axis that turns each pair; empty: positions are plain numbers
+    axes: int = 0        # of a position
 
     def __hash__(self):  # memoised plans: one object per set of arguments
         return id(self)
@@ -80,7 +107,7 @@ class RotaryPlan:
                 flush_retired_plans()
                 with device_context(device_index):
                     made = native.NativeRotary(self.frequencies, self.max_positions, self.amplitude, self.layout,
-                                               device_index)
+                                               device_index, self.axis_of)
                 hit = _NATIVE[key] = (weakref.ref(self, lambda _r: _drop(key, _r)), made)
         return hit[1]
 
@@ -112,12 +139,32 @@ def _number(name: str, v) -> float:
     return float(v)
 
 
+def _axis_of(axes: RotaryAxes, pairs: int) -> tuple:
+    """(axis, place among the axis' own pairs) of each pair."""
+    if not isinstance(axes, RotaryAxes):
+        raise TypeError(f"axes must be a RotaryAxes, got {type(axes).__name__}")
+    if not 1 <= len(axes.pairs) <= native.MAX_AXES or min(axes.pairs) < 1 or sum(axes.pairs) != pairs:
+        raise ValueError(f"axes.pairs must be 1 to {native.MAX_AXES} numbers of at least 1 that add up to the {pairs} "
+                         f"pairs of rot_dim, got {axes.pairs}")
+    if axes.order not in ("blocks", "cycle"):
+        raise ValueError(f"unknown axes.order {axes.order!r}: one of ['blocks', 'cycle']")
+    if axes.ladder not in ("own", "shared"):
+        raise ValueError(f"unknown axes.ladder {axes.ladder!r}: one of ['own', 'shared']")
+    out = [(a, i) for a, n in enumerate(axes.pairs) for i in range(n)]
+    # in turn: all axes' first pairs, then all their second ones
+    return tuple(out if axes.order == "blocks" else sorted(out, key=lambda p: (p[1], p[0])))
+
+
 @functools.lru_cache(maxsize=256, typed=True)
 def plan_rotary(head_dim: int, rot_dim: int | None = None, layout: str = "half", base: float = 10000.0,
-                scaling: RotaryScaling | None = None, max_positions: int = 1 << 20) -> RotaryPlan:
+                scaling: RotaryScaling | None = None, max_positions: int = 1 << 20,
+                axes: RotaryAxes | None = None) -> RotaryPlan:
     """Resolve a rotation (host-only, no torch; the same arguments give the
     same plan).  ``layout`` says which channels form pair ``j``: ``"half"``
-    ``(j, j + rot_dim / 2)``, ``"interleaved"`` ``(2 j, 2 j + 1)``."""
+    ``(j, j + rot_dim / 2)``, ``"interleaved"`` ``(2 j, 2 j + 1)``.  With
+    ``axes`` positions have several axes, each in ``[0, max_positions)``, and
+    ``scaling`` goes by each pair's own frequency (kind ``"base"``: by the
+    ladder that it stands on)."""
     if _whole("head_dim", head_dim) < 2 or head_dim % 2:
         raise ValueError(f"head_dim must be even and at least 2, got {head_dim}")
     r = head_dim if rot_dim is None else _whole("rot_dim", rot_dim)
@@ -128,6 +175,13 @@ def plan_rotary(head_dim: int, rot_dim: int | None = None, layout: str = "half",
     if not 1 <= _whole("max_positions", max_positions) <= MAX_POSITIONS_LIMIT:
         raise ValueError(f"max_positions must be in [1, {MAX_POSITIONS_LIMIT}], got {max_positions}")
     base = _number("base", base)
+    pair_axes = None if axes is None else _axis_of(axes, r // 2)
+    # pair j stands on step `step` of a ladder of `of` pairs
+    if axes is not None and axes.ladder == "own":
+        steps = [(i, axes.pairs[a]) for a, i in pair_axes]
+    else:
+        steps = [(j, r // 2) for j in range(r // 2)]
+    bases = [base] * (r // 2)
     amplitude = 1.0
     if scaling is not None:
         if not isinstance(scaling, RotaryScaling):
@@ -135,10 +189,11 @@ def plan_rotary(head_dim: int, rot_dim: int | None = None, layout: str = "half",
         factor = _number("scaling.factor", scaling.factor)
         amplitude = _number("scaling.amplitude", scaling.amplitude)
         if scaling.kind == "base":
-            if r == 2:
-                raise ValueError("scaling kind 'base' needs rot_dim > 2")
-            base *= factor ** (r / (r - 2))
-    theta = [base ** (-2.0 * j / r) for j in range(r // 2)]
+            if min(of for _, of in steps) == 1:
+                raise ValueError("scaling kind 'base' needs rot_dim > 2" if axes is None or axes.ladder != "own" else
+                                 "scaling kind 'base' needs two pairs or more of each axis")
+            bases = [base * factor ** (of / (of - 1)) for _, of in steps]
+    theta = [b ** (-2.0 * j / (2 * of)) for b, (j, of) in zip(bases, steps)]
     if scaling is not None and scaling.kind == "linear":
         theta = [t / factor for t in theta]
     elif scaling is not None and scaling.kind == "parts":
@@ -153,7 +208,8 @@ def plan_rotary(head_dim: int, rot_dim: int | None = None, layout: str = "half",
             theta[j] = t * (keep + (1.0 - keep) / factor)
     elif scaling is not None and scaling.kind != "base":
         raise ValueError(f"unknown scaling kind {scaling.kind!r}: one of ['base', 'linear', 'parts']")
-    return RotaryPlan(head_dim, r, layout, tuple(theta), amplitude, max_positions)
+    return RotaryPlan(head_dim, r, layout, tuple(theta), amplitude, max_positions,
+                      *(() if axes is None else (tuple(a for a, _ in pair_axes), len(axes.pairs))))
 
 
 # the torch module, the dtype ids, the autograd function and the query for
@@ -204,26 +260,32 @@ def _launch(plan, x, positions, inverse, out):
     dev = x.get_device()
     if out is None:
         out = _torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    xs, os, ps = x.stride(), out.stride(), positions.stride()
+    xs, os, ps, between = x.stride(), out.stride(), positions.stride(), 0
+    if plan.axes:
+        between, ps = ps[0], ps[1:]
     if x.dim() == 3:
         batch, (tokens, heads, dim) = 1, x.shape
         xs, os, ps = (0,) + xs, (0,) + os, (0,) + ps
     else:
         batch, tokens, heads, dim = x.shape
-        if positions.dim() == 1:
+        if len(ps) == 1:
             ps = (0,) + ps
     args = native.ROTARY_ARGS.pack(
         x.data_ptr(), out.data_ptr(), positions.data_ptr(), xs[0], xs[1], xs[2], os[0], os[1], os[2], ps[0], ps[1],
         batch, tokens, heads, dim, _DTYPES[x.dtype], positions.dtype is _torch.int64,
         native.DIR_IDS["inverse" if inverse else "forward"])
     table = plan.native(dev)
+    if plan.axes:
+        execute, rest = native.rotary_execute_axes, (args, between)
+    else:
+        execute, rest = native.rotary_execute, (args,)
     if current_device() == dev:
-        native.rotary_execute(table, args, stream_handle(dev))
+        execute(table, *rest, stream_handle(dev))
     else:
         from .context import device_context
 
         with device_context(dev):
-            native.rotary_execute(table, args, stream_handle(dev))
+            execute(table, *rest, stream_handle(dev))
     return out
 
 
@@ -244,7 +306,13 @@ def _check(plan, x, positions, out):
     if x.shape[-1] != plan.head_dim:
         raise ValueError(f"plan expects head_dim {plan.head_dim}, got shape {tuple(x.shape)}")
     lead = tuple(x.shape[:-2])
-    if tuple(positions.shape) not in (lead, lead[-1:]):
+    if plan.axes:
+        every = (plan.axes,)
+        if tuple(positions.shape) not in (every + lead, every + lead[-1:]):
+            raise ValueError(f"positions must have shape {every + lead}"
+                             f"{' or ' + str(every + lead[-1:]) if len(lead) == 2 else ''} (the plan has {plan.axes} "
+                             f"axes), got {tuple(positions.shape)}")
+    elif tuple(positions.shape) not in (lead, lead[-1:]):
         raise ValueError(f"positions must have shape {lead}{' or ' + str(lead[-1:]) if len(lead) == 2 else ''}, got "
                          f"{tuple(positions.shape)}")
     if x.stride(-1) != 1:
@@ -268,8 +336,10 @@ def execute_rotary_plan(plan: RotaryPlan, x, positions, *, inverse: bool = False
     head_dim)`` (any strides with adjacent channels; float32, float16 or
     bfloat16, computed in 32 bits) by ``positions`` (``(tokens,)`` or
     ``(batch, tokens)``, int32 or int64) into a new tensor, or into ``out``,
-    which may be ``x`` itself.  A position outside ``[0, max_positions)``
-    gives NaN.  ``inverse=True`` multiplies by the conjugate roots.  Takes
+    which may be ``x`` itself.  Positions of a plan with axes have one more
+    dimension in front, ``(axes, tokens)`` or ``(axes, batch, tokens)``.  A
+    position outside ``[0, max_positions)`` gives NaN (in the pairs its axis
+    turns).  ``inverse=True`` multiplies by the conjugate roots.  Takes
     part in autograd, reverse and forward mode."""
     if _torch is None:
         _load_torch()
