@@ -468,6 +468,27 @@ typedef struct {
 int mfft_cache_attend_workspace(const mfft_cache* cache, const mfft_attend_args* args, int64_t* bytes);
 int mfft_cache_attend(const mfft_cache* cache, const mfft_attend_args* args, void* stream);
 
+/* The same with more said of the keys.
+ * sinks, with a window: a query also sees the first `sinks` keys of its
+ * sequence (with `causal`, up to its own position).  Pages that lie between
+ * the sinks and every query's window do not count, and may be others'.
+ * prefix_pages: sequences prefix_groups[g] .. prefix_groups[g + 1] begin with
+ * the same prefix_pages[g] pages, the same entries in each one's row of the
+ * page table as far as its length reaches.  The result is that without it;
+ * those pages are read once for all of a group's queries instead of once a
+ * sequence.  (With a window it is not used.)  The workspace then also holds
+ * 4 head_dim + 8 bytes for each query row. */
+typedef struct {
+    int64_t sinks;                /* 0: none */
+    const int32_t* prefix_pages;  /* [groups], or NULL */
+    const int32_t* prefix_groups; /* [groups + 1], rising, or NULL: one group of all sequences */
+    int32_t groups;
+} mfft_attend_options;
+int mfft_cache_attend_with_workspace(const mfft_cache* cache, const mfft_attend_args* args,
+                                     const mfft_attend_options* options, int64_t* bytes);
+int mfft_cache_attend_with(const mfft_cache* cache, const mfft_attend_args* args, const mfft_attend_options* options,
+                           void* stream);
+
 /* Device facts for the profile / environment fingerprint. */
 int mfft_device_props_get(int device, mfft_device_props* out);
 

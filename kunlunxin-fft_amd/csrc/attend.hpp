@@ -1,0 +1,98 @@
+// attend.hpp -- what the launches of attention over the paged cache and its
+// kernels share: which keys a launch is about, its shape, and what it leaves
+// for the next.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mfft_internal.hpp"
+
+namespace mfft {
+
+// The keys that a launch is about.
+//   kAll:    what its sequences' queries see, one run of keys for each query
+//   kSinks:  the same in a window, and the sequence's first `sinks` keys
+//   kPrefix: the keys that groups of sequences share, for all rows of a group;
+//            each row's m, l and O (unscaled) are left in `carry`
+//   kRest:   each sequence's keys after those, going on from `carry`
+enum Part { kAll, kSinks, kPrefix, kRest };
+
+// x / d of 0 <= x < 2^31, exact: with l the least so that d <= 2^l and
+// m = ceil(2^(31 + l) / d), floor(x m / 2^(31 + l)).  (A division by a number
+// that is no constant is about twenty instructions, and a 64-bit one a hundred
+// and fifty; code that runs once a launch is mostly time to fetch it.)
+struct Divisor {
+    uint32_t m, shift;
+};
+inline Divisor divisor(uint32_t d) {
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < d) ++l;
+    return {(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), 31 + l};
+}
+
+struct AttendShape {
+    int group;        // query heads a key head
+    Divisor by_group, by_heads;
+    int rows, log_rows;  // rows of a block, a power of two
+    int units;        // page_size / 16
+    uint64_t magic;   // floor(2^32 / units) + 1: x / units = x * magic >> 32, exact for x < 2^26
+    int grid;         // shares; 0: one workgroup an item, none cut
+    int least;        // fewest groups of 64 keys in a share
+    int live;         // rows of a block that can be in use
+    int join_rows;    // rows of a workgroup of the join
+    int64_t per;      // queries of each sequence without offsets
+    // kSinks
+    int sinks;        // keys that stay visible
+    // kPrefix, kRest
+    int groups;                   // of sequences
+    const int32_t* prefix_pages;  // [groups]
+    const int32_t* prefix_groups; // [groups + 1], NULL: one group of all sequences
+    float* carry_o;               // [tokens][q_heads][head_dim]
+    float2* carry_ml;             // [tokens][q_heads]
+};
+
+constexpr int kCUs = 256;
+constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
+// Up to here, times the items there are for each workgroup at once, an item is
+// never cut: the second launch costs more than it saves, and many items balance
+// by themselves.  One token a sequence of 32 query and 8 key heads of 128,
+// lengths to the one given (several sequences: mixed), in us, whole and cut:
+// 1 sequence of 1000 10.7 and 15.1, 2000 16.2 and 12.1, 4000 24.8 and 16.2;
+// 8 of 2000 16.2 and 17.0, 4000 26.1 and 19.8, 8000 45 and 34; 256 of 1000 55
+// and 111.  64 of 2000 and 4000, past the bound, would be faster whole: 30 and
+// 54, 55 and 68; of 8000 it is the same, 121.
+constexpr int kWholeTiles = 16;
+
+// the item that starts in share i and is cut at its end: its parts are in
+// slots 2 i + 1, 2 (i + 1), 2 (i + 2), ... of the workspace
+struct Cut {
+    int parts;  // 0: none
+    int b, block, h;
+};
+
+// The forms and the workgroups that a CU holds at once, by their registers and
+// LDS: O and Q are D R / 4 + D R / 8 registers a lane, and kKeys holds K and V
+// of the next group too.
+enum Form { kKeys1, kKeys2, kKeys4, kRows, kTall };
+constexpr int attend_per_cu(int d, Form f) {
+    return f == kKeys1 ? (d >= 256 ? 1 : 2) : f == kKeys2 ? (d >= 128 ? 1 : 2) : f == kKeys4 ? 1 : 2;
+}
+
+// Rows of no sequence are written by workgroups that have nothing else to do,
+// kIdle more than there may be work for: after the work of all workgroups,
+// 0.7 us were added to the shortest call.
+constexpr int kIdle = 32;
+
+struct AttendLaunch {
+    AttendShape sh;
+    Form form;
+    int64_t grid, o_bytes, ml_bytes, cut_bytes;
+    int idle;  // workgroups more than work, see clear_rest: of the join where there is one
+};
+
+// One part's launches (attend_<part>_kernels.hip); workspace: args->workspace.
+template <Part PART>
+void launch_part(const mfft_cache& c, const mfft_attend_args& a, const AttendLaunch& w, hipStream_t s);
+
+}  // namespace mfft

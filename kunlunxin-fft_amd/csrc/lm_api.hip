@@ -370,17 +370,30 @@ static int check_attend(const mfft_cache* c, const mfft_attend_args* a) {
     return MFFT_OK;
 }
 
-int mfft_cache_attend_workspace(const mfft_cache* c, const mfft_attend_args* a, int64_t* bytes) {
-    mfft::clear_error();
-    if (!bytes) return fail(MFFT_ERR_VALUE, "bytes must not be NULL");
-    *bytes = 0;
-    if (int rc = check_attend(c, a)) return rc;
-    *bytes = a->tokens ? mfft::attend_workspace(*c, *a) : 0;
+static int check_options(const mfft_attend_options* o) {
+    if (!o) return fail(MFFT_ERR_VALUE, "options must not be NULL");
+    if (o->sinks < 0 || o->sinks > (int64_t)1 << 30) return fail(MFFT_ERR_VALUE, "sinks must be in [0, 2^30]");
+    if (o->prefix_pages) {
+        if (o->groups < 1 || (!o->prefix_groups && o->groups != 1))
+            return fail(MFFT_ERR_VALUE, "prefix_pages must be of one group at least, and of one only without prefix_groups, got %d",
+                        o->groups);
+        if (!aligned(o->prefix_pages, 4) || !aligned(o->prefix_groups, 4))
+            return fail(MFFT_ERR_VALUE, "prefix_pages and prefix_groups must be 4-byte aligned");
+    } else if (o->prefix_groups) {
+        return fail(MFFT_ERR_VALUE, "prefix_groups say whose prefix_pages are: give prefix_pages");
+    }
     return MFFT_OK;
 }
 
-int mfft_cache_attend(const mfft_cache* c, const mfft_attend_args* a, void* stream) {
-    mfft::clear_error();
+static int workspace(const mfft_cache* c, const mfft_attend_args* a, const mfft_attend_options& o, int64_t* bytes) {
+    if (!bytes) return fail(MFFT_ERR_VALUE, "bytes must not be NULL");
+    *bytes = 0;
+    if (int rc = check_attend(c, a)) return rc;
+    *bytes = a->tokens ? mfft::attend_workspace(*c, *a, o) : 0;
+    return MFFT_OK;
+}
+
+static int attend(const mfft_cache* c, const mfft_attend_args* a, const mfft_attend_options& opt, void* stream) {
     if (int rc = check_attend(c, a)) return rc;
     if (a->tokens == 0) return MFFT_OK;
     const int64_t D = c->head_dim;
@@ -395,17 +408,40 @@ int mfft_cache_attend(const mfft_cache* c, const mfft_attend_args* a, void* stre
     const Extent o = extent(a->out, {a->tokens, (int64_t)a->q_heads}, a->out_strides, D, 2);
     if (overlap(extent(a->q, {a->tokens, (int64_t)a->q_heads}, a->q_strides, D, 2), o))
         return fail(MFFT_ERR_VALUE, "q and out must not overlap");
-    if (!mfft::attend_launch_fits(*c, *a))
+    if (!mfft::attend_launch_fits(*c, *a, opt))
         return fail(MFFT_ERR_UNSUPPORTED, "%lld tokens need a launch of 2^32 work-items or more; split the call", (long long)a->tokens);
-    const int64_t need = mfft::attend_workspace(*c, *a);
+    const int64_t need = mfft::attend_workspace(*c, *a, opt);
     if (need > 0) {
         if (!a->workspace || a->workspace_bytes < need)
             return fail(MFFT_ERR_VALUE, "the call needs %lld bytes of workspace, got %lld", (long long)need,
                         (long long)(a->workspace ? a->workspace_bytes : 0));
         if (!aligned(a->workspace, 256)) return fail(MFFT_ERR_VALUE, "workspace must be 256-byte aligned");
     }
-    const hipError_t e = mfft::launch_attend(*c, *a, (hipStream_t)stream);
+    const hipError_t e = mfft::launch_attend(*c, *a, opt, (hipStream_t)stream);
     return e == hipSuccess ? MFFT_OK : hip_fail(e, "kernel launch");
+}
+
+int mfft_cache_attend_workspace(const mfft_cache* c, const mfft_attend_args* a, int64_t* bytes) {
+    mfft::clear_error();
+    return workspace(c, a, mfft_attend_options{}, bytes);
+}
+
+int mfft_cache_attend_with_workspace(const mfft_cache* c, const mfft_attend_args* a, const mfft_attend_options* o,
+                                     int64_t* bytes) {
+    mfft::clear_error();
+    if (int rc = check_options(o)) return rc;
+    return workspace(c, a, *o, bytes);
+}
+
+int mfft_cache_attend(const mfft_cache* c, const mfft_attend_args* a, void* stream) {
+    mfft::clear_error();
+    return attend(c, a, mfft_attend_options{}, stream);
+}
+
+int mfft_cache_attend_with(const mfft_cache* c, const mfft_attend_args* a, const mfft_attend_options* o, void* stream) {
+    mfft::clear_error();
+    if (int rc = check_options(o)) return rc;
+    return attend(c, a, *o, stream);
 }
 
 }  // extern "C"

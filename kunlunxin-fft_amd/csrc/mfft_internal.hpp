@@ -200,9 +200,9 @@ bool append_launch_fits(const RotaryTables& t, const mfft_cache& c, const mfft_a
 hipError_t launch_read(const mfft_cache& c, const mfft_read_args& a, hipStream_t stream);
 bool read_launch_fits(const mfft_cache& c, const mfft_read_args& a);
 bool attend_supported(int head_dim);
-bool attend_launch_fits(const mfft_cache& c, const mfft_attend_args& a);
-int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a);
-hipError_t launch_attend(const mfft_cache& c, const mfft_attend_args& a, hipStream_t stream);
+bool attend_launch_fits(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o);
+int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o);
+hipError_t launch_attend(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o, hipStream_t stream);
 
 }  // namespace mfft
 

@@ -46,6 +46,7 @@ EXPORTS = (
     "mfft_rotary_create_axes", "mfft_rotary_execute_axes",
     "mfft_cache_append", "mfft_cache_append_at", "mfft_cache_read",
     "mfft_cache_attend_workspace", "mfft_cache_attend",
+    "mfft_cache_attend_with_workspace", "mfft_cache_attend_with",
 )
 PLAN_CALLER_WORKSPACE = 1
 
@@ -59,6 +60,7 @@ CACHE_ARGS = struct.Struct("@4Pq3i4x")
 APPEND_ARGS = struct.Struct("@4P8q3P2q4i")
 ATTEND_ARGS = struct.Struct("@3P4q3P2q4ifi2qPq")
 READ_ARGS = struct.Struct("@2P4q3P2q3i4x")
+ATTEND_OPTIONS = struct.Struct("@q2Pi4x")
 MAX_AXES = 4
 
 
@@ -169,6 +171,11 @@ def load() -> ctypes.CDLL:
         lib.mfft_cache_attend_workspace.restype = i32
         lib.mfft_cache_attend.argtypes = [ctypes.c_char_p, ctypes.c_char_p, vp]
         lib.mfft_cache_attend.restype = i32
+        lib.mfft_cache_attend_with_workspace.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p,
+                                                         ctypes.POINTER(i64)]
+        lib.mfft_cache_attend_with_workspace.restype = i32
+        lib.mfft_cache_attend_with.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, vp]
+        lib.mfft_cache_attend_with.restype = i32
         lib.mfft_last_error.argtypes = []
         lib.mfft_last_error.restype = ctypes.c_char_p
         lib.mfft_abi_version.argtypes = []
@@ -388,6 +395,18 @@ def cache_attend_workspace(cache: bytes, args: bytes) -> int:
 
 def cache_attend(cache: bytes, args: bytes, stream_ptr: int) -> None:
     rc = load().mfft_cache_attend(cache, args, stream_ptr)
+    if rc:
+        check(rc)
+
+
+def cache_attend_with_workspace(cache: bytes, args: bytes, options: bytes) -> int:
+    k = ctypes.c_int64(0)
+    check(load().mfft_cache_attend_with_workspace(cache, args, options, ctypes.byref(k)))
+    return k.value
+
+
+def cache_attend_with(cache: bytes, args: bytes, options: bytes, stream_ptr: int) -> None:
+    rc = load().mfft_cache_attend_with(cache, args, options, stream_ptr)
     if rc:
         check(rc)
 

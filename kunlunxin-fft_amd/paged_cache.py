@@ -295,9 +295,26 @@ def read_paged_cache(cache: PagedCache, page_table, starts, tokens: int, *, offs
     return k, v
 
 
+def _prefixes(cache, pages, groups) -> int:
+    """Checks what groups of sequences share; how many groups there are."""
+    if pages is None:
+        if groups is not None:
+            raise ValueError("prefix_groups say whose prefix_pages are: give prefix_pages")
+        return 0
+    _index("prefix_pages", pages, cache.device, 1)
+    n = pages.shape[0]
+    if n < 1 or (groups is None and n != 1):
+        raise ValueError(f"prefix_pages must have an entry for each group (without prefix_groups one), got {n}")
+    if groups is not None:
+        _index("prefix_groups", groups, cache.device, 1)
+        if groups.shape[0] != n + 1:
+            raise ValueError(f"prefix_groups must have {n + 1} entries, got {groups.shape[0]}")
+    return n
+
+
 def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=None, scale: float | None = None,
                        causal: bool = True, window: int | None = None, max_length: int | None = None,
-                       return_lse: bool = False):
+                       return_lse: bool = False, sinks: int = 0, prefix_pages=None, prefix_groups=None):
     """Attention of ``q`` ``(tokens, q_heads, head_dim)`` (float16 or bfloat16;
     ``q_heads`` a multiple of the cache's) over the cache: ``softmax(scale q k)
     v``, a new tensor of ``q``'s shape and type.  Scores, maxima and sums are
@@ -307,8 +324,11 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
     Sequence ``b``'s queries are rows ``offsets[b] .. offsets[b + 1]`` (None:
     as many for every sequence) and are the last of its ``lengths[b]``
     positions.  ``causal``: a query sees the keys up to its own position;
-    ``window``: only that many of the last ones.  A query that sees no key, or
-    is no sequence's (padding before the first offset or past the last), gives 0.
+    ``window``: only that many of the last ones, and with it ``sinks``: the
+    sequence's first ``sinks`` keys too (pages that no window reaches do not
+    count then, and may have been given to others).  A query that sees no key,
+    or is no sequence's (padding before the first offset or past the last),
+    gives 0.
     ``scale`` defaults to ``head_dim ** -0.5``.  ``max_length``, if given,
     bounds ``lengths`` and lets short calls run in one launch; a longer
     sequence is still computed.  ``return_lse``: also the logarithm of the sum
@@ -316,6 +336,15 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
     A sequence longer than its table's pages, or with a page number that is not
     one of the cache's, gives NaN.  Takes no part in autograd: a ``q`` that
     requires a gradient is refused unless under ``torch.no_grad()``.
+
+    ``prefix_pages`` ``(groups,)``: sequences ``prefix_groups[g] ..
+    prefix_groups[g + 1]`` begin with the same ``prefix_pages[g]`` pages, the
+    same entries of their rows of ``page_table`` as far as each one's length
+    reaches (``prefix_groups`` ``(groups + 1,)``, rising; None: one group of all
+    sequences; sequences of no group share nothing).  The result is the one
+    without, but for the order of sums; the pages are read once for all of a
+    group's queries.  Both are int32 on the cache's device.  With a window
+    they are not used.
     """
     _sequences(cache, page_table, lengths, "lengths", offsets)
     _heads("q", q, cache)
@@ -331,6 +360,9 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
         raise ValueError(f"window must be None or an int in [1, {_MAX_POSITIONS}], got {window!r}")
     if max_length is not None and (isinstance(max_length, bool) or not isinstance(max_length, int) or max_length < 0):
         raise ValueError(f"max_length must be None or an int of at least 0, got {max_length!r}")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or not 0 <= sinks <= _MAX_POSITIONS:
+        raise ValueError(f"sinks must be an int in [0, {_MAX_POSITIONS}], got {sinks!r}")
+    groups = _prefixes(cache, prefix_pages, prefix_groups)
     scale = cache.head_dim ** -0.5 if scale is None else _scale(scale)
     _no_gradient("q", q)
     _gpu(cache)
@@ -345,12 +377,22 @@ def attend_paged_cache(cache: PagedCache, q, page_table, lengths, *, offsets=Non
             page_table.stride(0), tokens, page_table.shape[1], lengths.shape[0], heads, _DTYPES[q.dtype],
             scale, bool(causal), window or 0, 0 if max_length is None else min(max_length, _MAX_POSITIONS), ws, nbytes)
 
+    options = None
+    if sinks or groups:
+        options = native.ATTEND_OPTIONS.pack(sinks, 0 if prefix_pages is None else prefix_pages.data_ptr(),
+                                             0 if prefix_groups is None else prefix_groups.data_ptr(), groups)
     with _ledger.phase("cache-attend"):
         args = pack(0, 0)
-        need = native.cache_attend_workspace(cache._packed, args)
+        if options is None:
+            need = native.cache_attend_workspace(cache._packed, args)
+        else:
+            need = native.cache_attend_with_workspace(cache._packed, args, options)
         if need:
             # this call's, from torch's stream-ordered allocator on this stream
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             args = pack(ws.data_ptr(), need)
-        _on_device(cache.device, native.cache_attend, cache._packed, args)
+        if options is None:
+            _on_device(cache.device, native.cache_attend, cache._packed, args)
+        else:
+            _on_device(cache.device, native.cache_attend_with, cache._packed, args, options)
     return (out, lse) if return_lse else out
