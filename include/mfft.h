@@ -422,7 +422,8 @@ int mfft_cache_append_at(const mfft_cache* cache, const mfft_rotary* rotary, con
 /* Cached tokens read back: rows offsets[b] .. offsets[b + 1] of k and v are
  * code * scale of positions starts[b], starts[b] + 1, ... of sequence b,
  * rounded to the type.  A position below 0 or past the table's width, and a
- * page number that is none, give NaN; rows of no sequence 0. */
+ * page number that is none, give NaN; rows of no sequence 0.  k and v 16-byte
+ * aligned, with strides that keep it so. */
 typedef struct {
     void* k;                   /* [tokens][kv_heads][head_dim] */
     void* v;

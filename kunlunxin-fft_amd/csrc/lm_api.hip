@@ -323,11 +323,12 @@ int mfft_cache_read(const mfft_cache* c, const mfft_read_args* a, void* stream) 
                     (long long)a->tokens, a->sequences);
     if (int rc = check_strides("k", {a->tokens, (int64_t)c->kv_heads}, a->k_strides)) return rc;
     if (int rc = check_strides("v", {a->tokens, (int64_t)c->kv_heads}, a->v_strides)) return rc;
-    if (int rc = check_device(nullptr)) return rc;
     if (a->tokens == 0) return MFFT_OK;
     const int es = dtype_size(a->dtype);
-    if (!a->k || !a->v || !aligned(a->k, es) || !aligned(a->v, es))
-        return fail(MFFT_ERR_VALUE, "k and v must not be NULL and be aligned to their elements");
+    // (the stride of one token, or of one head, is not used)
+    auto keeps = [&](const int64_t* st) { return (a->tokens == 1 || st[0] * es % 16 == 0) && (c->kv_heads == 1 || st[1] * es % 16 == 0); };
+    if (!a->k || !a->v || !aligned(a->k, 16) || !aligned(a->v, 16) || !keeps(a->k_strides) || !keeps(a->v_strides))
+        return fail(MFFT_ERR_VALUE, "k and v must not be NULL, and 16-byte aligned with strides that keep it so");
     if (!distinct({a->tokens, (int64_t)c->kv_heads}, a->k_strides, c->head_dim) ||
         !distinct({a->tokens, (int64_t)c->kv_heads}, a->v_strides, c->head_dim))
         return fail(MFFT_ERR_VALUE, "k's or v's strides make its elements overlap");

@@ -171,7 +171,9 @@ def test_c_entries_refuse_before_device_work():
     good = [p << 10, p << 11, 128, 64, 128, 64, p, p, 0, 2, 6, 2, 3, native.F16]
     for i, value, rc, text in ((13, 7, native.ERR_TYPE, b"type"), (10, 7, native.ERR_VALUE, b"as many"), (10, -1, native.ERR_VALUE, b"tokens"),
                                (12, 0, native.ERR_VALUE, b"sequences"), (11, 0, native.ERR_VALUE, b"column"), (6, 0, native.ERR_VALUE, b"NULL"),
-                               (7, 0, native.ERR_VALUE, b"NULL"), (8, p + 1, native.ERR_VALUE, b"offsets"), (2, -1, native.ERR_VALUE, b"stride")):
+                               (7, 0, native.ERR_VALUE, b"NULL"), (8, p + 1, native.ERR_VALUE, b"offsets"), (2, -1, native.ERR_VALUE, b"stride"),
+                               (2, 132, native.ERR_VALUE, b"aligned"), (0, (p << 10) + 8, native.ERR_VALUE, b"aligned"), (1, 0, native.ERR_VALUE, b"NULL"),
+                               (2, 64, native.ERR_VALUE, b"overlap"), (1, p << 10, native.ERR_VALUE, b"overlap"), (0, p + 64, native.ERR_VALUE, b"overlap")):
         v = list(good)
         v[i] = value
         assert lib.mfft_cache_read(cache, native.READ_ARGS.pack(*v), None) == rc, (i, value)
