@@ -21,6 +21,7 @@
 // the same chain of loads: 64 of a workgroup's 256 threads have a pair of a key
 // of 128 channels, and a page that grows is rescaled whole, filled or not.
 #include "lm_device.hpp"
+#include "mfft_device.hpp"
 
 namespace mfft {
 namespace {
@@ -72,11 +73,16 @@ __device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const m
     const bool turned = ch * V < t.pairs, half = t.layout == MFFT_ROTARY_HALF;
     const int d0 = turned && half ? ch * V : ch * 2 * V, d1 = turned && half ? d0 + t.pairs : d0 + V;
     float2 w[V];
-    if (turned)
+    if (turned) {
+        if constexpr (PLACED) {
+            const AxisRoots<V> root(t, places.p, places.wide, n * places.token_stride, places.axis_stride, ch * V);
 #pragma unroll
-        for (int x = 0; x < V; ++x)
-            w[x] = PLACED ? axis_root(t, places.p, places.wide, n * places.token_stride, places.axis_stride, ch * V + x)
-                          : rotary_root(t, p, ch * V + x);
+            for (int x = 0; x < V; ++x) w[x] = root(t, x);
+        } else {
+#pragma unroll
+            for (int x = 0; x < V; ++x) w[x] = rotary_root(t, p, ch * V + x);
+        }
+    }
     const E* x = (const E*)a.q + n * a.q_strides[0] + h0 * a.q_strides[1];
     E* y = (E*)a.q_out + n * a.q_out_strides[0] + h0 * a.q_out_strides[1];
     auto turn = [&](Vec& u, Vec& v) {
@@ -185,10 +191,14 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
     const int m = (int)(p1 - p0);       // tokens written
     const int64_t row = row0 + (p0 - start);
 
-    // root of pair e of the i-th of these tokens
-    auto root = [&](int i, int e) {
-        if constexpr (PLACED) return axis_root(t, places.p, places.wide, (row + i) * places.token_stride, places.axis_stride, e);
-        else return rotary_root(t, p0 + i, e);
+    // root(x) is the root of pair e + x, x < n, of the i-th of these tokens
+    auto roots = [&](int i, int e, auto n) {
+        if constexpr (PLACED) {
+            const AxisRoots<decltype(n)::value> root(t, places.p, places.wide, (row + i) * places.token_stride, places.axis_stride, e);
+            return [&t, root](int x) { return root(t, x); };
+        } else {
+            return [&t, p = p0 + i, e](int x) { return rotary_root(t, p, e + x); };
+        }
     };
     const E* k = (const E*)a.k + row * a.k_strides[0] + h * a.k_strides[1];
     const E* v = (const E*)a.v + row * a.v_strides[0] + h * a.v_strides[1];
@@ -262,9 +272,10 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
             }
             if (!turned) return;
             const bool half = t.layout == MFFT_ROTARY_HALF;
+            const auto root = roots(tok, ch * V, ic<V>{});
 #pragma unroll
             for (int x = 0; x < V; ++x) {
-                const float2 r = root(tok, ch * V + x);
+                const float2 r = root(x);
                 // pairs (x, V + x), or (2 x, 2 x + 1)
                 const float fa = half ? f[x] : f[2 * x], fb = half ? f[V + x] : f[2 * x + 1];
                 const float2 y = rotate_pair({fa, fb}, r);
@@ -361,7 +372,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
         pair_channels(t.layout, t.pairs, e, d0, d1);
         const float fa = to_float(k[i * a.k_strides[0] + d0]), fb = to_float(k[i * a.k_strides[0] + d1]);
         if (e >= t.pairs) return make_float2(fa, fb);
-        return rotate_pair({fa, fb}, root(i, e));
+        return rotate_pair({fa, fb}, roots(i, e, ic<1>{})(0));
     };
     float mk = 0.0f, mv = 0.0f;
     for (int i = threadIdx.x; i < m * half; i += 256) {

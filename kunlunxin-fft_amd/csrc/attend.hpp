@@ -41,11 +41,14 @@ struct AttendShape {
     int least;        // fewest groups of 64 keys in a share
     int live;         // rows of a block that can be in use
     int join_rows;    // rows of a workgroup of the join
+    int whole_tiles;  // kRest: items of up to as many groups of keys are never cut
+    int block_tokens; // kSinks: tokens of a sequence whose rows a block can have
     int64_t per;      // queries of each sequence without offsets
     // kSinks
     int sinks;        // keys that stay visible
     // kPrefix, kRest
     int groups;                   // of sequences
+    int64_t items;                // kPrefix: that `cuts` has room for
     const int32_t* prefix_pages;  // [groups]
     const int32_t* prefix_groups; // [groups + 1], NULL: one group of all sequences
     float* carry_o;               // [tokens][q_heads][head_dim]
@@ -66,6 +69,7 @@ constexpr int kWholeTiles = 16;
 
 // the item that starts in share i and is cut at its end: its parts are in
 // slots 2 i + 1, 2 (i + 1), 2 (i + 2), ... of the workspace
+// (kPrefix, whose items are few: in the order of items, `h` its share)
 struct Cut {
     int parts;  // 0: none
     int b, block, h;
@@ -87,7 +91,7 @@ constexpr int kIdle = 32;
 struct AttendLaunch {
     AttendShape sh;
     Form form;
-    int64_t grid, o_bytes, ml_bytes, cut_bytes;
+    int64_t grid, join_grid, o_bytes, ml_bytes, cut_bytes;
     int idle;  // workgroups more than work, see clear_rest: of the join where there is one
 };
 

@@ -230,7 +230,6 @@ struct Sequence {
     bool poison;      // it has more than the table's
     int low, tiles;   // first key that any query sees (a multiple of 64), groups of 64 keys in the list
     int blocks;       // of rows
-    int sink_tiles;   // kSinks: groups of 64 keys, from the first on, that come before `low`'s
     int prefix;       // kRest: keys that are not its own
     int first, last;  // kPrefix: its sequences
 };
@@ -271,10 +270,6 @@ __device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_att
         const int lo = q.len - q.n + 1 - (int)a.window;
         q.low = lo > 0 ? lo & ~63 : 0;
     }
-    if constexpr (PART == kSinks) {
-        q.sink_tiles = (sh.sinks + 63) >> 6;
-        if (64 * q.sink_tiles >= q.low) q.sink_tiles = q.low = 0;
-    }
     if constexpr (PART == kRest) {
         // the last group that starts at or before b
         int g = 0, hi = sh.groups - 1;
@@ -286,7 +281,13 @@ __device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_att
         if (group_start(a, sh, g) <= b && b < group_start(a, sh, g + 1)) q.prefix = prefix_keys(c, a, sh, g);
         q.low = min(q.prefix, q.len) & ~63;
     }
-    q.tiles = q.sink_tiles + ((q.len - q.low + 63) >> 6);
+    q.tiles = (q.len - q.low + 63) >> 6;
+    if constexpr (PART == kSinks) {
+        // of a block: its own rows' windows and the sinks, not all the sequence's
+        const int tokens = min(sh.block_tokens, q.n);
+        if (a.causal) q.tiles = min(q.tiles, ((int)a.window + tokens + 62 + 63) >> 6);
+        q.tiles = min(q.tiles + ((sh.sinks + 63) >> 6), (q.len + 63) >> 6);
+    }
     if (q.tiles < 1) q.tiles = 1;  // rows that see nothing are still written
     q.blocks = (q.n * sh.group + sh.rows - 1) >> sh.log_rows;
     return q;
@@ -354,6 +355,7 @@ struct WorkList {
     const AttendShape& sh;
     bool by_item;
     int64_t w, upto;  // of the 64 sequences at hand: this lane's, and with those before
+    int most = 0;     // kRest: this lane's longest item
 
     __device__ __forceinline__ int count() const { return PART == kPrefix ? sh.groups : a.sequences; }
     __device__ __forceinline__ void take(int i) {
@@ -362,6 +364,7 @@ struct WorkList {
         if (b < count()) {
             const Sequence q = sequence<PART>(c, a, sh, b);
             w = (int64_t)q.blocks * c.kv_heads * (by_item ? 1 : q.tiles);
+            if (PART == kRest && q.blocks > 0) most = max(most, q.tiles);
         }
         upto = wave_scan(w);
     }
@@ -415,7 +418,7 @@ struct Item {
         return a.window ? max(seq.len - seq.n + tok + 1 - (int)a.window, 0) : 0;
     }
     __device__ __forceinline__ int upper(int tok) const {
-        if constexpr (PART == kPrefix) {  // of its own sequence, as far as they are shared
+        if constexpr (PART == kPrefix) {  // of its own sequence, as far as they are shared; 0: see `blind`
             int lo = seq.first, hi = seq.last - 1;
             if (!a.offsets) lo = (int)((seq.row0 + tok) / sh.per);
             else
@@ -437,9 +440,10 @@ struct Item {
     // kSinks: of rows that see [.., top) the keys [0, sink_keys(top)) too
     __device__ __forceinline__ int sink_keys(int top) const { return PART == kSinks ? min(sh.sinks, top) : 0; }
 
-    // The keys of groups [tile, upto) of the list that rows of the block see, as
-    // one run [from, end) of places; the place of a key is its number, and from
-    // `split` on (kSinks: the sinks' groups come first) less `gap`.
+    // The keys of groups [tile, upto) of the item's list that rows of the block
+    // see, as one run [from, end) of places.  The place of a key is its number;
+    // kSinks: the sinks' groups come first and the block's windows follow, from
+    // `split` on, their numbers less `gap`.
     int split, gap;
     __device__ __forceinline__ int key_at(int place) const { return PART != kSinks || place < split ? place : place + gap; }
     __device__ __forceinline__ void span(int tile, int upto, int& from, int& end) {
@@ -448,14 +452,10 @@ struct Item {
             end = min(seq.low + 64 * upto, block_hi);
             return;
         }
-        const int s = seq.sink_tiles, sinks_end = min((sink_keys(block_hi) + 63) & ~63, block_lo & ~63);
-        int b0 = seq.low + 64 * (max(tile, s) - s), b1 = seq.low + 64 * (max(upto, s) - s);
-        from = s ? 64 * min(tile, s) : b0;
-        split = max(min(s ? 64 * min(upto, s) : b1, sinks_end), from);
-        b0 = max(b0, block_lo & ~63);
-        b1 = min(b1, block_hi);
-        gap = b0 - split;
-        end = split + max(b1 - b0, 0);
+        split = min((sink_keys(block_hi) + 63) & ~63, block_lo & ~63);
+        gap = (block_lo & ~63) - split;
+        from = 64 * tile;
+        end = min(64 * upto, block_hi - gap);
     }
 
     __device__ __forceinline__ void take(int b, int block_, int h_, int rows) {
@@ -466,14 +466,15 @@ struct Item {
         if constexpr (PART == kPrefix) {
             // The shared pages stand in all its sequences' rows of the table; taken
             // are those of the longest (an empty one may name none).  The least
-            // that a row of the group sees bounds what all rows of the block see.
+            // that a row sees, blind ones left out, bounds what all of the block's
+            // see: a sequence's first row, or 1 where that comes before its keys.
             int64_t longest = -1;
             int least = seq.len;
             for (int s = seq.first + (int)(threadIdx.x & 63); s < seq.last; s += 64) {
                 const int row = (int)seq_offset(a.offsets, sh.per, a.tokens, s);
                 const int len = min(max(a.lengths[s], 0), a.table_width * c.page_size);
                 longest = max(longest, (int64_t)len << 32 | (uint32_t)(0x7fffffff - s));
-                if ((int)seq_offset(a.offsets, sh.per, a.tokens, s + 1) > row) least = min(least, seen_by(s, row));
+                if (len > 0 && (int)seq_offset(a.offsets, sh.per, a.tokens, s + 1) > row) least = min(least, max(seen_by(s, row), 1));
             }
 #pragma unroll
             for (int s = 1; s < 64; s <<= 1) {
@@ -573,6 +574,10 @@ struct Attend : Item<D, PART> {
     f32x4 o[R][S::N];
     float m[R], l[R];
     bool large;                        // some row's maximum has been past kFusedScores
+    // kPrefix: rows that see none of the keys (of an empty place in a batch, say)
+    // go through the loop as if they saw all, so that a group's other rows need no
+    // masks, and are cleared at its end
+    bool blind[R];
 
     // of the group at hand
     u32x4 kw[4][S::J > 0 ? S::J : 1];
@@ -611,7 +616,12 @@ struct Attend : Item<D, PART> {
                 qv[r.value][2 * jj.value + 1] = *(const x8*)(q + 64 * jj.value + 16 * g + 8);
             });
             if constexpr (S::REM) qv[r.value][S::KK - 1] = *(const x8*)(q + 64 * S::J + 8 * g);
-            const int lo = this->lower(tok), hi = max(this->upper(tok), lo);
+            const int lo = this->lower(tok);
+            int hi = max(this->upper(tok), lo);
+            if constexpr (PART == kPrefix) {
+                blind[r.value] = hi == 0;
+                if (hi == 0) hi = this->block_hi;
+            }
             low[r.value] = lo;
             top[r.value] = hi;
             all_lo = max(all_lo, lo);
@@ -636,6 +646,15 @@ struct Attend : Item<D, PART> {
         any_hi = __builtin_amdgcn_readfirstlane(any_hi);
     }
 
+    __device__ __forceinline__ void clear_blind() {
+        static_for<0, R>([&](auto r) {
+            if (blind[r.value]) {
+                m[r.value] = kLowest;
+                l[r.value] = 0.0f;
+                static_for<0, S::N>([&](auto i) { o[r.value][i.value] = f32x4{0, 0, 0, 0}; });
+            }
+        });
+    }
     // kRest: the shared keys' m, l and O, for the part of the item that has its
     // first key
     __device__ __forceinline__ void carry_in() {
@@ -969,6 +988,7 @@ struct Attend : Item<D, PART> {
         this->span(tile, upto, from, end);
         if constexpr (KEYS) run_keys(from, end);
         else run_rows(from, end);
+        if constexpr (PART == kPrefix) clear_blind();
     }
 
     // ---- out of the registers
@@ -1048,6 +1068,7 @@ struct Tall : Item<D, PART> {
     f32x16 o[D / 32];
     float m, l;
     bool large;  // some row's maximum has been past kFusedScores
+    bool blind;  // see Attend
 
     __device__ __forceinline__ Tall(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
         : I(c_, a_, sh_), lds(lds_) {
@@ -1067,6 +1088,10 @@ struct Tall : Item<D, PART> {
         static_for<0, D / 16>([&](auto i) { qv[i.value] = *(const x8*)(q + 16 * i.value); });
         low = this->lower(tok);
         top = max(this->upper(tok), low);
+        if constexpr (PART == kPrefix) {
+            blind = top == 0;
+            if (blind) top = this->block_hi;
+        }
         all_lo = any_lo = low;
         all_hi = any_hi = top;
 #pragma unroll
@@ -1283,6 +1308,13 @@ struct Tall : Item<D, PART> {
         nan_left = lds.nan != 0;
         mark_nans(from, end);
         l += __shfl_xor(l, 32);
+        if constexpr (PART == kPrefix) {
+            if (blind) {
+                m = kLowest;
+                l = 0.0f;
+                static_for<0, D / 32>([&](auto i) { static_for<0, 16>([&](auto x) { o[i.value][x.value] = 0.0f; }); });
+            }
+        }
     }
 
     __device__ __forceinline__ void mark_nans(int from, int end) {
@@ -1388,24 +1420,41 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
     // groups [at, stop) of the list; with one workgroup an item, of that item
     int64_t before, at = 0, stop, share = INT64_MAX;
     int b, item, tile = 0;
-    if (sh.grid == 0) {
-        b = WorkList<PART>{c, a, sh, true, 0, 0}.find(blockIdx.x, before, false);
+    WorkList<PART> list{c, a, sh, sh.grid == 0, 0, 0};
+    int64_t total = 0;
+    bool whole = sh.grid == 0;
+    if (!whole) {
+        total = list.total();
+        if constexpr (PART == kRest) {
+            // how long items are only the device knows: one workgroup an item then
+            // too, none cut (attend_launch has workgroups enough for that)
+            int most = list.most;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) most = max(most, __shfl_xor(most, s));
+            whole = uniform(most) <= sh.whole_tiles;
+            if (whole && (int)blockIdx.x < sh.grid && threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
+            list.by_item = whole;
+            if (!whole && (int)blockIdx.x >= sh.grid) return;
+        }
+    }
+    if (whole) {
+        b = list.find(blockIdx.x, before, false);
         if (b < 0) {
-            if constexpr (PART != kPrefix) clear_rest<E, D>(a, blockIdx.x - before, gridDim.x - before);
+            if constexpr (PART != kPrefix) {
+                if (sh.grid == 0) clear_rest<E, D>(a, blockIdx.x - before, gridDim.x - before);
+            }
             return;
         }
         w.seq = sequence<PART>(c, a, sh, b);
         item = (int)((int64_t)blockIdx.x - before);
         stop = w.seq.tiles;
     } else {
-        WorkList<PART> list{c, a, sh, false, 0, 0};
-        const int64_t total = list.total();
         const int64_t even = quotient(total + sh.grid - 1, sh.grid);
         share = even > sh.least ? even : sh.least;
         at = blockIdx.x * share;
         stop = at + share < total ? at + share : total;
         if (at >= stop) {
-            if (threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
+            if (PART != kPrefix && threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
             return;
         }
         b = list.find(at, before, list.count() <= 64);
@@ -1413,6 +1462,14 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
         const int64_t i = quotient(at - before, w.seq.tiles);
         item = (int)i;
         tile = (int)(at - before - i * w.seq.tiles);
+    }
+    // kPrefix: which of all items this is, whose cut is cuts[] of that
+    int64_t number = 0;
+    if constexpr (PART == kPrefix) {
+        if (sh.grid) {
+            for (int g = (int)(threadIdx.x & 63); g < b; g += 64) number += sequence<PART>(c, a, sh, g).blocks;
+            number = from_lane(wave_scan(number), 63) * c.kv_heads + item;
+        }
     }
     Cut cut{0, 0, 0, 0};
     while (true) {
@@ -1425,16 +1482,19 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
         w.run(tile, upto);
         if (tile == 0 && upto == w.seq.tiles) {
             w.store();
+            if (PART == kPrefix && sh.grid && threadIdx.x == 0 && number < sh.items) cuts[number].parts = 0;
         } else {
             w.store_part(2 * (int)blockIdx.x + (tile == 0 ? 1 : 0), part_o, part_ml);
             if (tile == 0) {  // its last group lies `past` groups past this share's end
                 const int past = (int)(at + w.seq.tiles - 1 - stop);
-                cut = {share > past ? 2 : past / (int)share + 2, b, block, h};
+                cut = {share > past ? 2 : past / (int)share + 2, b, block, PART == kPrefix ? (int)blockIdx.x : h};
+                if (PART == kPrefix && threadIdx.x == 0 && number < sh.items) cuts[number] = cut;
             }
         }
         at += upto - tile;
         if (at >= stop) break;
         tile = 0;
+        ++number;
         if (++item == w.seq.blocks * c.kv_heads) {
             item = 0;
             do {  // there is one: work is left
@@ -1442,7 +1502,7 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
             } while (w.seq.blocks == 0);
         }
     }
-    if (sh.grid && threadIdx.x == 0) cuts[blockIdx.x] = cut;
+    if (PART != kPrefix && !whole && threadIdx.x == 0) cuts[blockIdx.x] = cut;
 }
 
 // Cut items, `sh.join_rows` rows a workgroup: of few parts, a wave a row; of
@@ -1453,17 +1513,25 @@ __global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_arg
                                                    const float2* part_ml, const Cut* cuts) {
     constexpr int C = (D + 63) / 64;
     const int groups = (sh.live + sh.join_rows - 1) / sh.join_rows;
-    const int share = blockIdx.x / groups;
-    if (share >= sh.grid) {
-        if constexpr (PART != kPrefix) clear_rest<E, D>(a, blockIdx.x - sh.grid * groups, gridDim.x - sh.grid * groups);
+    int share = blockIdx.x / groups;
+    int64_t before = 0;
+    if constexpr (PART == kPrefix) {  // an item's number
+        if (WorkList<PART>{c, a, sh, true, 0, 0}.find(share, before, false) < 0) return;
+    } else if (share >= sh.grid) {
+        clear_rest<E, D>(a, blockIdx.x - sh.grid * groups, gridDim.x - sh.grid * groups);
         return;
     }
-    const Cut cut = cuts[share];
+    Cut cut = cuts[share];
     if (cut.parts == 0) return;
+    if constexpr (PART == kPrefix) {
+        const int item = (int)(share - before);
+        share = cut.h;
+        cut.h = item - item / sh.by_heads * c.kv_heads;
+    }
     const Sequence seq = sequence<PART>(c, a, sh, cut.b);
     const int block = cut.block * sh.rows, all = seq.n * sh.group;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool wide = cut.parts > 8;
+    const bool wide = PART != kPrefix && cut.parts > 8;
     const int first = (int)(blockIdx.x % groups) * sh.join_rows;
     const int end = min(min(first + sh.join_rows, sh.live), all - block);
     __shared__ float sl[4], so[4][64 * C];
@@ -1532,7 +1600,7 @@ void launch_dim(const mfft_cache& c, const mfft_attend_args& a, const AttendLaun
     }
     mark(s);
     if (w.sh.grid) {
-        join_kernel<E, D, PART><<<w.sh.grid * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows) + w.idle, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+        join_kernel<E, D, PART><<<(uint32_t)w.join_grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
         mark(s);
     }
 }

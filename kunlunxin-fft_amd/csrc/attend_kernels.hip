@@ -45,6 +45,7 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     // a cut costs its rows' partial sums, written and read again: about a
     // quarter as many groups of keys as it has rows
     w.sh.least = w.sh.rows / 4 > kLeastTiles ? w.sh.rows / 4 : kLeastTiles;
+    if (part == kPrefix) w.sh.least = kLeastTiles;
     w.sh.log_rows = ilog2(w.sh.rows);
     w.sh.by_group = divisor(w.sh.group);
     w.sh.by_heads = divisor(c.kv_heads);
@@ -53,7 +54,9 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     const int64_t at_once = kCUs * attend_per_cu(D, w.form);
     const int64_t table = (int64_t)a.table_width * c.page_size;
     int64_t longest = a.max_length && a.max_length < table ? a.max_length : table;
-    if (part == kSinks) longest = std::min(longest, o.sinks + a.window + a.tokens / sequences + 128);
+    w.sh.block_tokens = (w.sh.rows - 1) / w.sh.group + 2;
+    if (part == kSinks && a.causal)
+        longest = std::min(longest, ((o.sinks + 63) & ~(int64_t)63) + a.window + std::min<int64_t>(w.sh.block_tokens, a.tokens) + 126);
     const int64_t each = std::max<int64_t>(1, std::max<int64_t>(sequences, a.tokens * w.sh.group / w.sh.rows) * c.kv_heads / at_once);
     const bool whole = longest <= 64 * kWholeTiles * each;
     w.idle = a.offsets && part != kPrefix ? kIdle : 0;
@@ -62,11 +65,20 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
         // as many shares as workgroups run at once
         w.sh.grid = (int)at_once;
         w.grid = w.sh.grid;
+        if (part == kRest) {
+            w.sh.whole_tiles = (int)std::min<int64_t>(kWholeTiles * each, 1 << 20);
+            w.grid = std::max<int64_t>(w.grid, items);
+        }
         // few sequences and heads: their items are cut into many parts
         w.sh.join_rows = w.sh.live <= 16 && w.sh.grid >= 8 * (int64_t)sequences * c.kv_heads ? 1 : w.sh.live > 16 ? 8 : 4;
         w.o_bytes = (int64_t)2 * w.sh.grid * w.sh.rows * D * 4;
         w.ml_bytes = (int64_t)2 * w.sh.grid * w.sh.rows * 8;
-        w.cut_bytes = w.sh.grid * sizeof(Cut);
+        // kPrefix: items, few and long, by number (more than `items` only in groups
+        // that overlap, which are none)
+        if (part == kPrefix) w.sh.join_rows = 4;
+        w.sh.items = part == kPrefix ? items : w.sh.grid;
+        w.cut_bytes = w.sh.items * (int64_t)sizeof(Cut);
+        w.join_grid = w.sh.items * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows) + w.idle;
     }
     return w;
 }
@@ -88,9 +100,11 @@ int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a, const m
 }
 
 bool attend_launch_fits(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o) {
-    if (with_prefix(a, o))
-        return launch_fits(attend_launch(c, a, o, kPrefix).grid, 256) && launch_fits(attend_launch(c, a, o, kRest).grid, 256);
-    return launch_fits(attend_launch(c, a, o, with_sinks(a, o) ? kSinks : kAll).grid, 256);
+    auto fits = [&](Part part) {
+        const AttendLaunch w = attend_launch(c, a, o, part);
+        return launch_fits(std::max(w.grid, w.join_grid), 256);
+    };
+    return with_prefix(a, o) ? fits(kPrefix) && fits(kRest) : fits(with_sinks(a, o) ? kSinks : kAll);
 }
 
 hipError_t launch_attend(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o, hipStream_t stream) {

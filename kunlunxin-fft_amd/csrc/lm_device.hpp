@@ -52,6 +52,29 @@ __device__ __forceinline__ float2 axis_root(const RotaryTables& t, const void* p
     return rotary_root(t, position(p, wide, at + x * axis_stride), j);
 }
 
+// The roots of C pairs of one token, from pair j on (C a power of two, j a
+// multiple of it): its position along each axis is loaded once.
+template <int C>
+struct AxisRoots {
+    int64_t at[MFFT_MAX_AXES];
+    struct alignas(C) {
+        uint8_t of[C];
+    } axis;
+    int j;
+    __device__ __forceinline__ AxisRoots(const RotaryTables& t, const void* p, int32_t wide, int64_t place,
+                                         int64_t axis_stride, int j_) : axis{}, j(j_) {
+#pragma unroll
+        for (int x = 0; x < MFFT_MAX_AXES; ++x) at[x] = x == 0 || x < t.axes ? position(p, wide, place + x * axis_stride) : 0;
+        if (t.axes > 1) axis = *(const decltype(axis)*)(t.axis + j);
+    }
+    __device__ __forceinline__ float2 operator()(const RotaryTables& t, int x) const {
+        int64_t q = at[0];
+#pragma unroll
+        for (int y = 1; y < MFFT_MAX_AXES; ++y) q = axis.of[x] == y ? at[y] : q;
+        return rotary_root(t, q, j + x);
+    }
+};
+
 // Channels of pair e of a head: the rotated pairs first, then the rest two
 // by two.
 __device__ __forceinline__ void pair_channels(int layout, int pairs, int e, int& d0, int& d1) {

@@ -44,9 +44,9 @@ __global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_r
 // its chunk's roots and applies them to `heads` heads of one token, so that a
 // token's roots are loaded and multiplied once for them.  Channels past the
 // pairs are chunks of 2 V (V) copied.
-template <class E, bool HALF>
-__global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_rotary_args a, uint32_t chunks,
-                                                           uint32_t total, int heads) {
+template <class E, bool HALF, bool AXES>
+__global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_rotary_args a, int64_t axis_stride,
+                                                           uint32_t chunks, uint32_t total, int heads) {
     constexpr int V = 16 / sizeof(E), C = HALF ? V : V / 2;  // elements of a load, pairs of a chunk
     struct alignas(16) Vec {
         E e[V];
@@ -62,12 +62,18 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
     float2 w[C];
     if (turned) {
         const int64_t po = b * a.position_strides[0] + n * a.position_strides[1];
-        const int64_t p = position(a.positions, a.positions_64, po);
+        if constexpr (AXES) {
+            const AxisRoots<C> root(t, a.positions, a.positions_64, po, axis_stride, (int)c * C);
 #pragma unroll
-        for (int x = 0; x < C; ++x) {
-            w[x] = rotary_root(t, p, (int)c * C + x);
-            if (a.direction == MFFT_INVERSE) w[x].y = -w[x].y;
+            for (int x = 0; x < C; ++x) w[x] = root(t, x);
+        } else {
+            const int64_t p = position(a.positions, a.positions_64, po);
+#pragma unroll
+            for (int x = 0; x < C; ++x) w[x] = rotary_root(t, p, (int)c * C + x);
         }
+#pragma unroll
+        for (int x = 0; x < C; ++x)
+            if (a.direction == MFFT_INVERSE) w[x].y = -w[x].y;
     }
     const int h0 = blockIdx.y * heads, h1 = h0 + heads < a.heads ? h0 + heads : a.heads;
     const E* x = (const E*)a.in + b * a.in_strides[0] + n * a.in_strides[1] + h0 * a.in_strides[2];
@@ -132,14 +138,15 @@ int heads_a_thread(int64_t threads, int heads) {
 
 template <class E>
 void launch_type(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_stride, hipStream_t s) {
-    if (t.axes <= 1 && chunked(t, a)) {
+    if (chunked(t, a)) {
         const bool half = t.layout == MFFT_ROTARY_HALF;
         const uint32_t chunks = (uint32_t)(a.head_dim * sizeof(E) / (half ? 32 : 16));
         const uint32_t total = (uint32_t)(a.batch * a.tokens) * chunks;
         const int heads = heads_a_thread(total, a.heads);
         const dim3 grid((uint32_t)(((uint64_t)total + 255) / 256), (uint32_t)((a.heads + heads - 1) / heads));
-        if (half) rotary_chunk_kernel<E, true><<<grid, 256, 0, s>>>(t, a, chunks, total, heads);
-        else rotary_chunk_kernel<E, false><<<grid, 256, 0, s>>>(t, a, chunks, total, heads);
+        auto go = [&](auto* kernel) { kernel<<<grid, 256, 0, s>>>(t, a, axis_stride, chunks, total, heads); };
+        if (t.axes > 1) half ? go(rotary_chunk_kernel<E, true, true>) : go(rotary_chunk_kernel<E, false, true>);
+        else half ? go(rotary_chunk_kernel<E, true, false>) : go(rotary_chunk_kernel<E, false, false>);
         return;
     }
     const uint32_t half = (uint32_t)a.head_dim / 2;
