@@ -38,6 +38,7 @@ struct AppendGrid {
 // threads (four waves on each of 1024 SIMDs).
 constexpr int kQueryHeads = 16;
 
+template <bool PLACED>
 __host__ __device__ inline AppendGrid append_grid(const mfft_cache& c, const mfft_append_args& a, int v) {
     AppendGrid g;
     g.slots = a.offsets ? a.tokens / c.page_size + 2 * (int64_t)a.sequences : a.sequences;
@@ -47,45 +48,56 @@ __host__ __device__ inline AppendGrid append_grid(const mfft_cache& c, const mff
     g.q_heads = 1;
     while (v > 1 && g.q_heads < kQueryHeads && g.q_heads < a.q_heads && chunks * a.q_heads > ((int64_t)1 << 18) * g.q_heads) g.q_heads *= 2;
     g.q_slabs = a.q ? (a.q_heads + g.q_heads - 1) / g.q_heads : 0;
-    g.q_blocks = (chunks * g.q_slabs + 255) / 256;
+    const int per = 256 / (c.head_dim / (2 * v));  // whole tokens (pieces of their heads) of a workgroup
+    g.q_blocks = PLACED && v > 1 ? (a.tokens * g.q_slabs + per - 1) / per : (chunks * g.q_slabs + 255) / 256;
     return g;
 }
 
-// Queries: thread i takes V pairs of a token and `grid.q_heads` of its heads.
+// Queries: a thread takes V pairs of a token and `grid.q_heads` of its heads,
+// thread `i` of the grid the i-th.  With positions of their own, and V > 1, the
+// workgroup makes its tokens' roots together, in ws (and has whole tokens).
 template <class E, int V, bool PLACED>
-__device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& places,
-                             const AppendGrid& grid, int64_t at) {
+__device__ __forceinline__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a,
+                                             const Positions& places, const AppendGrid& grid, Divisor by_pairs, int64_t block,
+                                             float4* ws) {
     struct alignas(V * sizeof(E)) Vec {
         E e[V];
     };
-    const int chunks = c.head_dim / (2 * V);
-    const uint32_t i = (uint32_t)at;  // fewer than 2^32
-    const int ch = (int)(i % chunks);
-    const uint32_t ts = i / chunks;
-    const int64_t n = ts / (uint32_t)grid.q_slabs;
-    if (n >= a.tokens) return;
-    const int h0 = (int)(ts % (uint32_t)grid.q_slabs) * grid.q_heads, h1 = min(h0 + grid.q_heads, a.q_heads);
-    int64_t p = 0;
-    if constexpr (!PLACED) {
-        const int b = token_sequence(a.offsets, 1, a.tokens, a.sequences, n);
-        p = a.starts[b] + (n - seq_offset(a.offsets, 1, a.tokens, b));
-    }
+    constexpr bool TOGETHER = PLACED && V > 1;
+    const int chunks = c.head_dim / (2 * V), mine = (int)threadIdx.x / chunks;
+    const uint32_t i = (uint32_t)(block * 256 + threadIdx.x);  // fewer than 2^32
+    const int ch = TOGETHER ? (int)threadIdx.x - mine * chunks : (int)(i % chunks);
+    const uint32_t slabs = (uint32_t)grid.q_slabs, per = 256 / chunks;
+    const uint32_t ts = TOGETHER ? (uint32_t)block * per + mine : i / chunks;  // token and piece of its heads
+    const int64_t n = ts / slabs;
     const bool turned = ch * V < t.pairs, half = t.layout == MFFT_ROTARY_HALF;
     const int d0 = turned && half ? ch * V : ch * 2 * V, d1 = turned && half ? d0 + t.pairs : d0 + V;
     float2 w[V];
-    if (turned) {
+    if constexpr (TOGETHER) {
+        const uint32_t all = (uint32_t)(a.tokens * grid.q_slabs), first = (uint32_t)block * per, n0 = first / slabs;
+        const int count = (int)(min(first + per, all) - 1) / (int)slabs - (int)n0 + 1;  // of `per` at most
+        stage_roots<V>(t, ws, count, chunks, by_pairs, false, [&](int tok, int axis) {
+            return held_position(t, position(places.p, places.wide, (n0 + tok) * places.token_stride + axis * places.axis_stride));
+        });
+        __syncthreads();
+        if (mine >= (int)per || ts >= all) return;
+        if (turned) staged_roots<V>(ws, (int)(n - n0) * chunks + ch, w);
+    } else {
+        if (n >= a.tokens) return;
         if constexpr (PLACED) {
-            const AxisRoots<V> root(t, places.p, places.wide, n * places.token_stride, places.axis_stride, ch * V);
-#pragma unroll
-            for (int x = 0; x < V; ++x) w[x] = root(t, x);
+            if (turned) w[0] = AxisRoots<1>(t, places.p, places.wide, n * places.token_stride, places.axis_stride, ch)(0);
         } else {
+            const int b = token_sequence(a.offsets, 1, a.tokens, a.sequences, n);
+            const int64_t p = a.starts[b] + (n - seq_offset(a.offsets, 1, a.tokens, b));
+            if (turned)
 #pragma unroll
-            for (int x = 0; x < V; ++x) w[x] = rotary_root(t, p, ch * V + x);
+                for (int x = 0; x < V; ++x) w[x] = rotary_root(t, p, ch * V + x);
         }
     }
+    const int h0 = (int)(ts % slabs) * grid.q_heads, h1 = min(h0 + grid.q_heads, a.q_heads);
     const E* x = (const E*)a.q + n * a.q_strides[0] + h0 * a.q_strides[1];
     E* y = (E*)a.q_out + n * a.q_out_strides[0] + h0 * a.q_out_strides[1];
-    auto turn = [&](Vec& u, Vec& v) {
+    auto turn = [&](Vec& u, Vec& v) __attribute__((always_inline)) {
         if (!turned) return;
         E f[2 * V];
 #pragma unroll
@@ -97,7 +109,7 @@ __device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const m
         for (int z = 0; z < V; ++z) {
             const float fa = to_float(half ? f[z] : f[2 * z]), fb = to_float(half ? f[V + z] : f[2 * z + 1]);
             const float2 to = rotate_pair({fa, fb}, w[z]);
-            const E ra = from_float<E>(to.x), rb = from_float<E>(to.y);
+            const E ra = rounded_channel<E>(to.x), rb = rounded_channel<E>(to.y);
             if (half) {
                 u.e[z] = ra;
                 v.e[z] = rb;
@@ -132,6 +144,10 @@ __device__ void rotate_query(const RotaryTables& t, const mfft_cache& c, const m
     }
 }
 
+// a or b, both of them values: a choice between two elements of an array would
+// keep the array in memory
+__device__ __forceinline__ float pick(bool c, float a, float b) { return c ? a : b; }
+
 // four codes times a factor
 __device__ __forceinline__ uint32_t scale_codes(uint32_t w, float f) {
     uint32_t r = 0;
@@ -153,11 +169,13 @@ __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d)
 
 // PLACED: tokens are turned by positions of their own, not by their places.
 template <class E, bool WIDE, bool PLACED>
-__global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache c, mfft_append_args a, Positions places) {
+__global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache c, mfft_append_args a, Positions places,
+                                                     Divisor by_pairs) {
     constexpr int W = WIDE ? 16 / (int)sizeof(E) : 1;
-    const AppendGrid grid = append_grid(c, a, W);
+    const AppendGrid grid = append_grid<PLACED>(c, a, W);
+    __shared__ float4 ws[WIDE && PLACED ? W / 2 * 256 : 1];
     if ((int64_t)blockIdx.x >= grid.kv_blocks) {
-        rotate_query<E, W, PLACED>(t, c, a, places, grid, ((int64_t)blockIdx.x - grid.kv_blocks) * 256 + threadIdx.x);
+        rotate_query<E, W, PLACED>(t, c, a, places, grid, by_pairs, (int64_t)blockIdx.x - grid.kv_blocks, ws);
         return;
     }
     const int64_t slot = blockIdx.x / c.kv_heads;
@@ -194,8 +212,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
     // root(x) is the root of pair e + x, x < n, of the i-th of these tokens
     auto roots = [&](int i, int e, auto n) {
         if constexpr (PLACED) {
-            const AxisRoots<decltype(n)::value> root(t, places.p, places.wide, (row + i) * places.token_stride, places.axis_stride, e);
-            return [&t, root](int x) { return root(t, x); };
+            return AxisRoots<decltype(n)::value>(t, places.p, places.wide, (row + i) * places.token_stride, places.axis_stride, e);
         } else {
             return [&t, p = p0 + i, e](int x) { return rotary_root(t, p, e + x); };
         }
@@ -260,7 +277,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
             }
             return turned;
         };
-        auto key = [&](int i, float (&f)[2 * V]) {
+        auto key = [&](int i, float (&f)[2 * V]) __attribute__((always_inline)) {
             const int tok = i / half_chunks, ch = i % half_chunks;
             int d0, d1;
             const bool turned = channels(ch, d0, d1);
@@ -273,31 +290,27 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
             if (!turned) return;
             const bool half = t.layout == MFFT_ROTARY_HALF;
             const auto root = roots(tok, ch * V, ic<V>{});
+            float one[V], two[V];  // the turned pairs
 #pragma unroll
             for (int x = 0; x < V; ++x) {
-                const float2 r = root(x);
                 // pairs (x, V + x), or (2 x, 2 x + 1)
-                const float fa = half ? f[x] : f[2 * x], fb = half ? f[V + x] : f[2 * x + 1];
-                const float2 y = rotate_pair({fa, fb}, r);
-                if (half) {
-                    f[x] = y.x;
-                    f[V + x] = y.y;
-                } else {
-                    f[2 * x] = y.x;
-                    f[2 * x + 1] = y.y;
-                }
+                const float2 y = rotate_pair({pick(half, f[x], f[2 * x]), pick(half, f[V + x], f[2 * x + 1])}, root(x));
+                one[x] = y.x;
+                two[x] = y.y;
             }
+#pragma unroll
+            for (int x = 0; x < 2 * V; ++x)
+                f[x] = pick(half, x < V ? one[x % V] : two[x % V], x % 2 ? two[x / 2] : one[x / 2]);
         };
         float mk = 0.0f, mv = 0.0f;
-#pragma unroll
-        for (int r = 0; r < KEEP; ++r) {
-            const int i = threadIdx.x + 256 * r;
+        static_for<0, KEEP>([&](auto r) __attribute__((always_inline)) {
+            const int i = threadIdx.x + 256 * r.value;
             if (i < m * half_chunks) {
-                key(i, held[r]);
+                key(i, held[r.value]);
 #pragma unroll
-                for (int x = 0; x < 2 * V; ++x) mk = __builtin_fmaxf(mk, finite_abs(held[r][x]));
+                for (int x = 0; x < 2 * V; ++x) mk = __builtin_fmaxf(mk, finite_abs(held[r.value][x]));
             }
-        }
+        });
         for (int i = threadIdx.x + 256 * KEEP; i < m * half_chunks; i += 256) {
             float f[2 * V];
             key(i, f);
@@ -314,7 +327,7 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
         }
         settle(mk, mv);
         const float k_inv = 1.0f / k_new, v_inv = 1.0f / v_new;
-        auto write_key = [&](int i, const float (&f)[2 * V]) {
+        auto write_key = [&](int i, const float (&f)[2 * V]) __attribute__((always_inline)) {
             const int tok = i / half_chunks, ch = i % half_chunks;
             int d0, d1;
             (void)channels(ch, d0, d1);
@@ -325,11 +338,10 @@ __global__ __launch_bounds__(256) void append_kernel(RotaryTables t, mfft_cache 
                 *(uint32_t*)(kr + d1 + x) = to_codes(f[V + x] * k_inv, f[V + x + 1] * k_inv, f[V + x + 2] * k_inv, f[V + x + 3] * k_inv);
             }
         };
-#pragma unroll
-        for (int r = 0; r < KEEP; ++r) {
-            const int i = threadIdx.x + 256 * r;
-            if (r < rounds && i < m * half_chunks) write_key(i, held[r]);
-        }
+        static_for<0, KEEP>([&](auto r) __attribute__((always_inline)) {
+            const int i = threadIdx.x + 256 * r.value;
+            if (r.value < rounds && i < m * half_chunks) write_key(i, held[r.value]);
+        });
         for (int i = threadIdx.x + 256 * KEEP; i < m * half_chunks; i += 256) {
             float f[2 * V];
             key(i, f);
@@ -416,12 +428,13 @@ bool wide(const RotaryTables& t, const mfft_append_args& a) {
 
 template <class E, bool PLACED>
 void launch_form(const RotaryTables& t, const mfft_cache& c, const mfft_append_args& a, const Positions& at, hipStream_t s) {
+    const Divisor by = divisor(t.pairs > 0 ? t.pairs : 1);
     if (wide(t, a)) {
-        const AppendGrid g = append_grid(c, a, a.dtype == MFFT_F32 ? 4 : 8);
-        append_kernel<E, true, PLACED><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a, at);
+        const AppendGrid g = append_grid<PLACED>(c, a, a.dtype == MFFT_F32 ? 4 : 8);
+        append_kernel<E, true, PLACED><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a, at, by);
     } else {
-        const AppendGrid g = append_grid(c, a, 1);
-        append_kernel<E, false, PLACED><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a, at);
+        const AppendGrid g = append_grid<PLACED>(c, a, 1);
+        append_kernel<E, false, PLACED><<<(uint32_t)(g.kv_blocks + g.q_blocks), 256, 0, s>>>(t, c, a, at, by);
     }
 }
 
@@ -434,7 +447,7 @@ void launch_type(const RotaryTables& t, const mfft_cache& c, const mfft_append_a
 }  // namespace
 
 bool append_launch_fits(const RotaryTables&, const mfft_cache& c, const mfft_append_args& a) {
-    const AppendGrid g = append_grid(c, a, 1);
+    const AppendGrid g = append_grid<false>(c, a, 1);
     return launch_fits(g.kv_blocks + g.q_blocks, 256);
 }
 

@@ -18,19 +18,6 @@ namespace mfft {
 //   kRest:   each sequence's keys after those, going on from `carry`
 enum Part { kAll, kSinks, kPrefix, kRest };
 
-// x / d of 0 <= x < 2^31, exact: with l the least so that d <= 2^l and
-// m = ceil(2^(31 + l) / d), floor(x m / 2^(31 + l)).  (A division by a number
-// that is no constant is about twenty instructions, and a 64-bit one a hundred
-// and fifty; code that runs once a launch is mostly time to fetch it.)
-struct Divisor {
-    uint32_t m, shift;
-};
-inline Divisor divisor(uint32_t d) {
-    uint32_t l = 0;
-    while (((uint64_t)1 << l) < d) ++l;
-    return {(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), 31 + l};
-}
-
 struct AttendShape {
     int group;        // query heads a key head
     Divisor by_group, by_heads;

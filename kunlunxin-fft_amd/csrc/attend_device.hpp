@@ -222,8 +222,6 @@ __device__ __forceinline__ float log_sum(float m, float l, bool poison) {
 // lengths, which only the device knows; every workgroup works its place out for
 // itself with one pass of a wave over the sequences.  Cut items leave their
 // (m, l, O) in the workspace and join_kernel adds them up.
-__device__ __forceinline__ int operator/(int x, Divisor d) { return (int)((uint64_t)(uint32_t)x * d.m >> d.shift); }
-
 struct Sequence {
     int row0, n;      // its queries
     int len;          // its keys, within the table

@@ -151,8 +151,8 @@ static int create_rotary(mfft_rotary** out, const double* frequencies, const int
         };
         const std::vector<float2> lo = rows(lo_rows < max_positions ? lo_rows : max_positions, 1, 1.0L);
         const std::vector<float2> hi = rows(hi_rows, lo_rows, (long double)amplitude);
-        std::vector<float2> axis(axes > 1 ? (pairs + 7) / 8 : 0);
-        for (int j = 0; axes > 1 && j < pairs; ++j) ((uint8_t*)axis.data())[j] = (uint8_t)axis_of[j];
+        std::vector<float2> axis((pairs + 7) / 8);
+        for (int j = 0; axis_of && j < pairs; ++j) ((uint8_t*)axis.data())[j] = (uint8_t)axis_of[j];
         hipStream_t us = nullptr;
         int rc = MFFT_OK;
         hipError_t e = hipGetDevice(&r->device);
@@ -160,7 +160,7 @@ static int create_rotary(mfft_rotary** out, const double* frequencies, const int
         if (rc == MFFT_OK) rc = mfft::upload_stream(r->device, &us);
         if (rc == MFFT_OK) rc = mfft::upload(&r->lo, lo, &r->table_bytes, us);
         if (rc == MFFT_OK) rc = mfft::upload(&r->hi, hi, &r->table_bytes, us);
-        if (rc == MFFT_OK && axes > 1) rc = mfft::upload(&r->axis, axis, &r->table_bytes, us);
+        if (rc == MFFT_OK) rc = mfft::upload(&r->axis, axis, &r->table_bytes, us);
         if (us) {
             e = hipStreamSynchronize(us);  // also after a failure: the host tables die here
             if (e != hipSuccess && rc == MFFT_OK) rc = hip_fail(e, "hipStreamSynchronize(rotary tables)");

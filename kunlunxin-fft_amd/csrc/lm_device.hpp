@@ -31,8 +31,34 @@ __device__ __forceinline__ float2 rotate_pair(float2 x, float2 w) {
     return make_float2(__builtin_fmaf(x.x, w.x, -(x.y * w.y)), __builtin_fmaf(x.y, w.x, x.x * w.y));
 }
 
-// The root of position p, pair j.  p < 0 or past the table: NaN, so that a
-// position the plan does not hold shows in the output.
+// A channel of rotate_pair in the element type.  In float16 the last fma and the
+// conversion are one instruction, which rounds once; conversions of two
+// neighbours at a time are not, and round twice, so each is kept by itself.
+template <class E>
+__device__ __forceinline__ E rounded_channel(float v) {
+    E r = (E)v;
+    if constexpr (__is_same(E, _Float16)) asm("" : "+v"(r));
+    return r;
+}
+
+// A position as the tables are indexed: kNoPosition if the plan does not hold it.
+constexpr uint32_t kNoPosition = 0xffffffff;
+__device__ __forceinline__ uint32_t held_position(const RotaryTables& t, int64_t p) {
+    return (uint64_t)p < (uint64_t)t.max_positions ? (uint32_t)p : kNoPosition;
+}
+
+// The root of a held position, pair j; NaN of one that is not, so that it shows
+// in the output.  Loaded whatever the position is: a branch around a load ends
+// in a wait for it, and a thread needs roots of several positions at once.  (32
+// bits hold both tables' indexes: 2^24 positions, 256 pairs.)
+__device__ __forceinline__ float2 held_root(const RotaryTables& t, uint32_t p, int j) {
+    const uint32_t q = p == kNoPosition ? 0 : p, pairs = (uint32_t)t.pairs;
+    const float2 a = t.lo[(q & ((1u << kRotaryLoLog2) - 1)) * pairs + (uint32_t)j];
+    const float2 b = t.hi[(q >> kRotaryLoLog2) * pairs + (uint32_t)j];
+    const float2 z = rotate_pair(a, b);
+    return p == kNoPosition ? make_float2(__builtin_nanf(""), __builtin_nanf("")) : z;
+}
+// The same of one position for all of a thread's pairs: one branch for them.
 __device__ __forceinline__ float2 rotary_root(const RotaryTables& t, int64_t p, int j) {
     if (p < 0 || p >= t.max_positions) return make_float2(__builtin_nanf(""), __builtin_nanf(""));
     const float2 a = t.lo[(p & ((1 << kRotaryLoLog2) - 1)) * t.pairs + j];
@@ -43,37 +69,92 @@ __device__ __forceinline__ float2 rotary_root(const RotaryTables& t, int64_t p, 
 __device__ __forceinline__ int64_t position(const void* p, int32_t wide, int64_t at) {
     return wide ? ((const int64_t*)p)[at] : ((const int32_t*)p)[at];
 }
-
-// The root of pair j of the token whose positions stand from p[at] on, with
-// several axes.
-__device__ __forceinline__ float2 axis_root(const RotaryTables& t, const void* p, int32_t wide, int64_t at,
-                                            int64_t axis_stride, int j) {
-    const int x = t.axes > 1 ? t.axis[j] : 0;
-    return rotary_root(t, position(p, wide, at + x * axis_stride), j);
-}
+__device__ __forceinline__ int operator/(int x, Divisor d) { return (int)((uint64_t)(uint32_t)x * d.m >> d.shift); }
 
 // The roots of C pairs of one token, from pair j on (C a power of two, j a
-// multiple of it): its position along each axis is loaded once.
+// multiple of it), each by its axis of the positions that stand from p[place]
+// on.  (Positions are chosen by bits, not from an array, which would be one in LDS.)
 template <int C>
 struct AxisRoots {
-    int64_t at[MFFT_MAX_AXES];
-    struct alignas(C) {
-        uint8_t of[C];
-    } axis;
+    static_assert(MFFT_MAX_AXES == 4);
+    const RotaryTables& t;
+    uint64_t axis;  // a byte a pair
+    uint32_t at0, to1, at2, to3;
     int j;
-    __device__ __forceinline__ AxisRoots(const RotaryTables& t, const void* p, int32_t wide, int64_t place,
-                                         int64_t axis_stride, int j_) : axis{}, j(j_) {
-#pragma unroll
-        for (int x = 0; x < MFFT_MAX_AXES; ++x) at[x] = x == 0 || x < t.axes ? position(p, wide, place + x * axis_stride) : 0;
-        if (t.axes > 1) axis = *(const decltype(axis)*)(t.axis + j);
+    __device__ __forceinline__ AxisRoots(const RotaryTables& t_, const void* p, int32_t wide, int64_t place,
+                                         int64_t axis_stride, int j_) : t(t_), j(j_) {
+        if constexpr (C == 8) axis = *(const uint64_t*)(t.axis + j);
+        else if constexpr (C == 4) axis = *(const uint32_t*)(t.axis + j);
+        else axis = t.axis[j];
+        // (of axes there are not, the first's again: no branches)
+        const int64_t s1 = t.axes > 1 ? place + axis_stride : place, s2 = t.axes > 2 ? place + 2 * axis_stride : place,
+                      s3 = t.axes > 3 ? place + 3 * axis_stride : place;
+        int64_t p0, p1, p2, p3;
+        auto load = [&](auto* from) {
+            p0 = from[place];
+            p1 = from[s1];
+            p2 = from[s2];
+            p3 = from[s3];
+        };
+        if (wide) load((const int64_t*)p);
+        else load((const int32_t*)p);
+        at0 = held_position(t, p0);
+        to1 = at0 ^ held_position(t, p1);
+        at2 = held_position(t, p2);
+        to3 = at2 ^ held_position(t, p3);
     }
-    __device__ __forceinline__ float2 operator()(const RotaryTables& t, int x) const {
-        int64_t q = at[0];
-#pragma unroll
-        for (int y = 1; y < MFFT_MAX_AXES; ++y) q = axis.of[x] == y ? at[y] : q;
-        return rotary_root(t, q, j + x);
+    __device__ __forceinline__ float2 operator()(int x) const {
+        const uint32_t a = (uint32_t)(axis >> (8 * x)), odd = 0u - (a & 1), high = 0u - (a >> 1 & 1);
+        const uint32_t lo = at0 ^ (to1 & odd), hi = at2 ^ (to3 & odd);
+        return held_root(t, lo ^ ((lo ^ hi) & high), j + x);
     }
 };
+
+// The roots of a workgroup's tokens, in LDS: a thread that takes C pairs of a
+// head (a chunk) would load them in C pieces of eight bytes, every lane from
+// lines of its own, and with few heads for each that is most of what the caches
+// deliver.  Here neighbouring lanes load neighbouring pairs, once for all
+// chunks and heads.  Root x of chunk c of token n is half x % 2 of
+// ws[(x / 2) * 256 + n * stride + c]: a chunk's own pieces, as adjacent threads
+// read them, are adjacent.  All 256 threads call it; tokens * stride <= 256,
+// and stride chunks hold at least all pairs.  at(n, axis): a token's held position.
+template <int C, class At>
+__device__ __forceinline__ void stage_roots(const RotaryTables& t, float4* ws, int tokens, int stride, Divisor by_pairs,
+                                            bool inverse, At&& at) {
+    const int n = tokens * t.pairs;
+    if (n <= 0) return;
+    uint32_t p[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+        const int r = min((int)threadIdx.x + 256 * k, n - 1), tok = r / by_pairs;
+        p[k] = at(tok, (int)t.axis[r - tok * t.pairs]);
+    }
+    float2 w[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+        const int r = min((int)threadIdx.x + 256 * k, n - 1), tok = r / by_pairs;
+        w[k] = held_root(t, p[k], r - tok * t.pairs);
+        if (inverse) w[k].y = -w[k].y;
+    }
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+        const int r = (int)threadIdx.x + 256 * k;
+        if (r < n) {
+            const int tok = r / by_pairs, j = r - tok * t.pairs;
+            ((float2*)ws)[2 * (j % C / 2 * 256 + tok * stride + j / C) + j % 2] = w[k];
+        }
+    }
+}
+// a chunk's, of slot n * stride + c
+template <int C>
+__device__ __forceinline__ void staged_roots(const float4* ws, int slot, float2 (&w)[C]) {
+#pragma unroll
+    for (int x = 0; x < C; x += 2) {
+        const float4 v = ws[x / 2 * 256 + slot];
+        w[x] = make_float2(v.x, v.y);
+        w[x + 1] = make_float2(v.z, v.w);
+    }
+}
 
 // Channels of pair e of a head: the rotated pairs first, then the rest two
 // by two.

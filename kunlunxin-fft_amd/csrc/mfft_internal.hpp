@@ -171,6 +171,19 @@ hipError_t launch_fourstep(int dir, const float2* src, float2* dst, char* fws, c
 hipError_t launch_fourstep_real(const float2* src, float2* dst, float2* work, const mfft_plan* p, float scale,
                                 hipStream_t stream);
 
+// x / d of 0 <= x < 2^31, exact: with l the least so that d <= 2^l and
+// m = ceil(2^(31 + l) / d), floor(x m / 2^(31 + l)).  (A division by a number
+// that is no constant is about twenty instructions, and a 64-bit one a hundred
+// and fifty; code that runs once a launch is mostly time to fetch it.)
+struct Divisor {
+    uint32_t m, shift;
+};
+inline Divisor divisor(uint32_t d) {
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < d) ++l;
+    return {(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), 31 + l};
+}
+
 // ---- rotary_kernels.hip, append_kernels.hip, read_kernels.hip, attend_kernels.hip
 // Roots m exp(i p theta_j) of a position p are the product of a row of `lo`
 // (p mod 1024) and one of `hi` (p / 1024): see mfft_rotary below.
@@ -181,8 +194,8 @@ struct RotaryTables {
     int64_t max_positions;  // 0: no rotation
     int32_t pairs;
     int32_t layout;
-    int32_t axes;           // of a position; 0 and 1: one
-    const uint8_t* axis;    // [pairs], with several axes: the one that turns each pair
+    int32_t axes;           // of a position
+    const uint8_t* axis;    // [pairs]: the one that turns each pair
 };
 // Positions that do not follow from a token's place: axis x of token n at
 // p[x * axis_stride + n * token_stride].
@@ -215,6 +228,6 @@ struct mfft_rotary {
     mfft::RotaryTables t{};
     float2* lo = nullptr;
     float2* hi = nullptr;
-    float2* axis = nullptr;  // bytes: the axis of each pair
+    float2* axis = nullptr;  // bytes
     int64_t table_bytes = 0;
 };

@@ -12,8 +12,10 @@
 namespace mfft {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // One thread per (token, head, pair), any strides, alignment and sizes.
-template <class E, bool AXES>
+template <class E>
 __global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_rotary_args a, int64_t axis_stride,
                                                           uint32_t half_dim, uint32_t total) {
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -28,12 +30,11 @@ __global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_r
     E* y = (E*)a.out + b * a.out_strides[0] + n * a.out_strides[1] + h * a.out_strides[2];
     E va = x[d0], vb = x[d1];
     if ((int)e < t.pairs) {
-        float2 w = AXES ? axis_root(t, a.positions, a.positions_64, po, axis_stride, (int)e)
-                        : rotary_root(t, position(a.positions, a.positions_64, po), (int)e);
+        float2 w = rotary_root(t, position(a.positions, a.positions_64, po + t.axis[e] * axis_stride), (int)e);
         if (a.direction == MFFT_INVERSE) w.y = -w.y;
         const float2 z = rotate_pair({to_float(va), to_float(vb)}, w);
-        va = from_float<E>(z.x);
-        vb = from_float<E>(z.y);
+        va = rounded_channel<E>(z.x);
+        vb = rounded_channel<E>(z.y);
     }
     y[d0] = va;
     y[d1] = vb;
@@ -44,9 +45,9 @@ __global__ __launch_bounds__(256) void rotary_pair_kernel(RotaryTables t, mfft_r
 // its chunk's roots and applies them to `heads` heads of one token, so that a
 // token's roots are loaded and multiplied once for them.  Channels past the
 // pairs are chunks of 2 V (V) copied.
-template <class E, bool HALF, bool AXES>
-__global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_rotary_args a, int64_t axis_stride,
-                                                           uint32_t chunks, uint32_t total, int heads) {
+template <class E, bool HALF>
+__global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_rotary_args a, uint32_t chunks,
+                                                           uint32_t total, int heads) {
     constexpr int V = 16 / sizeof(E), C = HALF ? V : V / 2;  // elements of a load, pairs of a chunk
     struct alignas(16) Vec {
         E e[V];
@@ -62,18 +63,12 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
     float2 w[C];
     if (turned) {
         const int64_t po = b * a.position_strides[0] + n * a.position_strides[1];
-        if constexpr (AXES) {
-            const AxisRoots<C> root(t, a.positions, a.positions_64, po, axis_stride, (int)c * C);
+        const int64_t p = position(a.positions, a.positions_64, po);
 #pragma unroll
-            for (int x = 0; x < C; ++x) w[x] = root(t, x);
-        } else {
-            const int64_t p = position(a.positions, a.positions_64, po);
-#pragma unroll
-            for (int x = 0; x < C; ++x) w[x] = rotary_root(t, p, (int)c * C + x);
-        }
-#pragma unroll
-        for (int x = 0; x < C; ++x)
+        for (int x = 0; x < C; ++x) {
+            w[x] = rotary_root(t, p, (int)c * C + x);
             if (a.direction == MFFT_INVERSE) w[x].y = -w[x].y;
+        }
     }
     const int h0 = blockIdx.y * heads, h1 = h0 + heads < a.heads ? h0 + heads : a.heads;
     const E* x = (const E*)a.in + b * a.in_strides[0] + n * a.in_strides[1] + h0 * a.in_strides[2];
@@ -85,8 +80,8 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
             E& ea = HALF ? u.e[k] : u.e[2 * k];
             E& eb = HALF ? v.e[k] : u.e[2 * k + 1];
             const float2 z = rotate_pair({to_float(ea), to_float(eb)}, w[k]);
-            ea = from_float<E>(z.x);
-            eb = from_float<E>(z.y);
+            ea = rounded_channel<E>(z.x);
+            eb = rounded_channel<E>(z.y);
         }
     };
     int h = h0;
@@ -117,11 +112,110 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
     }
 }
 
+// The same of positions with several axes, where a chunk's roots lie in rows of
+// their own: the workgroup makes its tokens' roots together.  Roots loaded by
+// each thread as above: 1024 tokens of 40 heads of 128 21 us, so 9.3 (plain
+// positions 7.5, and 9.3 made together, as they take one more round of loads);
+// 50001 of 16 heads of 64 in float32 97 and 85 us (4.8 TB/s).
+template <class E, bool HALF>
+__global__ __launch_bounds__(256) void rotary_axes_kernel(RotaryTables t, mfft_rotary_args a, int64_t axis_stride,
+                                                           int chunks, int tokens, Divisor by_pairs, int heads) {
+    constexpr int V = 16 / sizeof(E), C = HALF ? V : V / 2;  // elements of a load, pairs of a chunk
+    union Vec {
+        E e[V];
+        u32x4 w;
+    };
+    __shared__ float4 ws[C / 2 * 256];
+    // tokens of all batches, one after the other: this workgroup's first, how many
+    // it has, and this thread's (a thread past the last takes the last again, and
+    // stores nothing)
+    const uint32_t first = blockIdx.x * (uint32_t)tokens, all = (uint32_t)(a.batch * a.tokens);
+    const int count = (int)min((uint32_t)tokens, all - first);
+    const int mine = (int)threadIdx.x / chunks, c = (int)threadIdx.x - mine * chunks, tok = min(mine, count - 1);
+    auto place = [&](int tok, int64_t& b, int64_t& n) {
+        n = first + (uint32_t)tok;
+        b = 0;
+        if (a.batch > 1) {
+            b = (uint32_t)n / (uint32_t)a.tokens;
+            n -= b * a.tokens;
+        }
+    };
+    int64_t b, n;
+    place(tok, b, n);
+    const bool turned = c * C < t.pairs;
+    // first channels of the chunk's two (one) loads
+    const int d0 = !HALF || !turned ? c * (HALF ? 2 * V : V) : c * C;
+    const int d1 = turned ? d0 + t.pairs : d0 + V;
+    const int h0 = blockIdx.y * heads, h1 = h0 + heads < a.heads ? h0 + heads : a.heads;
+    const E* x = (const E*)a.in + b * a.in_strides[0] + n * a.in_strides[1] + h0 * a.in_strides[2];
+    E* y = (E*)a.out + b * a.out_strides[0] + n * a.out_strides[1] + h0 * a.out_strides[2];
+    // four heads' loads before their stores (in and out may be one tensor, so the
+    // compiler keeps the order written), the first four's before the roots, which
+    // are two loads one after the other
+    Vec u[4], v[4];
+    auto load = [&] {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            u[k] = *(const Vec*)(x + k * a.in_strides[2] + d0);
+            if constexpr (HALF) v[k] = *(const Vec*)(x + k * a.in_strides[2] + d1);
+        }
+    };
+    int h = h0;
+    if (h + 4 <= h1) load();
+    stage_roots<C>(t, ws, count, chunks, by_pairs, a.direction == MFFT_INVERSE, [&](int tok, int axis) {
+        int64_t b, n;
+        place(tok, b, n);
+        return held_position(t, position(a.positions, a.positions_64,
+                                         b * a.position_strides[0] + n * a.position_strides[1] + axis * axis_stride));
+    });
+    __syncthreads();
+    if (mine >= count) return;
+    float2 w[C];
+    if (turned) staged_roots<C>(ws, mine * chunks + c, w);
+    // (here they are first used: the compiler otherwise converts them, and so waits
+    // for them, before it asks for positions and roots)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        asm volatile("" : "+v"(u[k].w));
+        if constexpr (HALF) asm volatile("" : "+v"(v[k].w));
+    }
+    auto turn = [&](Vec& u, Vec& v) {
+        if (!turned) return;
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+            E& ea = HALF ? u.e[k] : u.e[2 * k];
+            E& eb = HALF ? v.e[k] : u.e[2 * k + 1];
+            const float2 z = rotate_pair({to_float(ea), to_float(eb)}, w[k]);
+            ea = rounded_channel<E>(z.x);
+            eb = rounded_channel<E>(z.y);
+        }
+    };
+    for (; h + 4 <= h1; h += 4) {
+        if (h > h0) load();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            turn(u[k], v[k]);
+            *(Vec*)(y + k * a.out_strides[2] + d0) = u[k];
+            if constexpr (HALF) *(Vec*)(y + k * a.out_strides[2] + d1) = v[k];
+        }
+        x += 4 * a.in_strides[2];
+        y += 4 * a.out_strides[2];
+    }
+    for (; h < h1; ++h, x += a.in_strides[2], y += a.out_strides[2]) {
+        Vec u = *(const Vec*)(x + d0), v;
+        if constexpr (HALF) v = *(const Vec*)(x + d1);
+        turn(u, v);
+        *(Vec*)(y + d0) = u;
+        if constexpr (HALF) *(Vec*)(y + d1) = v;
+    }
+}
+
 // Whether every load and store of rotary_chunk_kernel is 16-byte aligned.
 bool chunked(const RotaryTables& t, const mfft_rotary_args& a) {
     const int v = a.dtype == MFFT_F32 ? 4 : 8;
     const bool half = t.layout == MFFT_ROTARY_HALF;
     if (t.pairs % (half ? v : v / 2) || a.head_dim % (half ? 2 * v : v)) return false;
+    if (t.axes > 1 && a.head_dim / (half ? 2 * v : v) > 256) return false;  // a workgroup has whole tokens
     if (((uintptr_t)a.in | (uintptr_t)a.out) & 15) return false;
     for (int i = 0; i < 3; ++i)
         if (a.in_strides[i] % v || a.out_strides[i] % v) return false;
@@ -143,17 +237,24 @@ void launch_type(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_
         const uint32_t chunks = (uint32_t)(a.head_dim * sizeof(E) / (half ? 32 : 16));
         const uint32_t total = (uint32_t)(a.batch * a.tokens) * chunks;
         const int heads = heads_a_thread(total, a.heads);
-        const dim3 grid((uint32_t)(((uint64_t)total + 255) / 256), (uint32_t)((a.heads + heads - 1) / heads));
-        auto go = [&](auto* kernel) { kernel<<<grid, 256, 0, s>>>(t, a, axis_stride, chunks, total, heads); };
-        if (t.axes > 1) half ? go(rotary_chunk_kernel<E, true, true>) : go(rotary_chunk_kernel<E, false, true>);
-        else half ? go(rotary_chunk_kernel<E, true, false>) : go(rotary_chunk_kernel<E, false, false>);
+        const uint32_t slabs = (uint32_t)((a.heads + heads - 1) / heads);
+        if (t.axes > 1) {
+            const int64_t all = a.batch * a.tokens, tokens = 256 / chunks;
+            const dim3 grid((uint32_t)((all + tokens - 1) / tokens), slabs);
+            const Divisor by = divisor(t.pairs);
+            if (half) rotary_axes_kernel<E, true><<<grid, 256, 0, s>>>(t, a, axis_stride, (int)chunks, (int)tokens, by, heads);
+            else rotary_axes_kernel<E, false><<<grid, 256, 0, s>>>(t, a, axis_stride, (int)chunks, (int)tokens, by, heads);
+            return;
+        }
+        const dim3 grid((uint32_t)(((uint64_t)total + 255) / 256), slabs);
+        if (half) rotary_chunk_kernel<E, true><<<grid, 256, 0, s>>>(t, a, chunks, total, heads);
+        else rotary_chunk_kernel<E, false><<<grid, 256, 0, s>>>(t, a, chunks, total, heads);
         return;
     }
     const uint32_t half = (uint32_t)a.head_dim / 2;
     const uint32_t total = (uint32_t)(a.batch * a.tokens * a.heads) * half;
     const uint32_t grid = (uint32_t)(((uint64_t)total + 255) / 256);
-    if (t.axes > 1) rotary_pair_kernel<E, true><<<grid, 256, 0, s>>>(t, a, axis_stride, half, total);
-    else rotary_pair_kernel<E, false><<<grid, 256, 0, s>>>(t, a, 0, half, total);
+    rotary_pair_kernel<E><<<grid, 256, 0, s>>>(t, a, axis_stride, half, total);
 }
 
 }  // namespace

@@ -241,8 +241,9 @@ def _load_torch():
 
         @staticmethod
         def backward(ctx, grad):
-            # again a Rotate, so that gradients of gradients work
-            return Rotate.apply(adjacent(grad), ctx.saved_tensors[0], ctx.plan, not ctx.inverse), None, None, None
+            # again a Rotate where it is differentiated in turn
+            turn = Rotate.apply if torch.is_grad_enabled() or runner.has_tangent(grad) else _turned
+            return turn(adjacent(grad), ctx.saved_tensors[0], ctx.plan, not ctx.inverse), None, None, None
 
         @staticmethod
         def jvp(ctx, tangent, *_):
@@ -252,6 +253,10 @@ def _load_torch():
     _Rotate = Rotate
     _has_tangent = runner.has_tangent
     _torch = torch
+
+
+def _turned(x, positions, plan, inverse):
+    return _launch(plan, x, positions, inverse, None)
 
 
 def _launch(plan, x, positions, inverse, out):
