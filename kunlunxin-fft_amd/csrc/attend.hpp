@@ -14,13 +14,22 @@ namespace mfft {
 //   kAll:    what its sequences' queries see, one run of keys for each query
 //   kSinks:  the same in a window, and the sequence's first `sinks` keys
 //   kPrefix: the keys that groups of sequences share, for all rows of a group;
-//            each row's m, l and O (unscaled) are left in `carry`
-//   kRest:   each sequence's keys after those, going on from `carry`
+//            each row's m, l and O (unscaled) are left in `carry`, or, of items
+//            that were cut, in the parts' workspace
+//   kRest:   each sequence's keys after those, going on from there
 enum Part { kAll, kSinks, kPrefix, kRest };
+
+// the item that starts in share i and is cut at its end: its parts are in
+// slots 2 i + 1, 2 (i + 1), 2 (i + 2), ... of the workspace
+// (kPrefix: not in the order of shares but of items, `h` the share)
+struct Cut {
+    int parts;  // 0: none
+    int b, block, h;
+};
 
 struct AttendShape {
     int group;        // query heads a key head
-    Divisor by_group, by_heads;
+    Divisor by_group, by_heads, by_per;
     int rows, log_rows;  // rows of a block, a power of two
     int units;        // page_size / 16
     uint64_t magic;   // floor(2^32 / units) + 1: x / units = x * magic >> 32, exact for x < 2^26
@@ -28,18 +37,24 @@ struct AttendShape {
     int least;        // fewest groups of 64 keys in a share
     int live;         // rows of a block that can be in use
     int join_rows;    // rows of a workgroup of the join
-    int whole_tiles;  // kRest: items of up to as many groups of keys are never cut
+    int whole_tiles, whole_more;  // kRest: see kAloneTiles
     int block_tokens; // kSinks: tokens of a sequence whose rows a block can have
     int64_t per;      // queries of each sequence without offsets
     // kSinks
     int sinks;        // keys that stay visible
     // kPrefix, kRest
     int groups;                   // of sequences
-    int64_t items;                // kPrefix: that `cuts` has room for
     const int32_t* prefix_pages;  // [groups]
     const int32_t* prefix_groups; // [groups + 1], NULL: one group of all sequences
     float* carry_o;               // [tokens][q_heads][head_dim]
     float2* carry_ml;             // [tokens][q_heads]
+    struct {                      // of kPrefix
+        int log_rows, grid;
+        int64_t items;            // that `cuts`, in the order of items, has room for
+        const Cut* cuts;          // kRest: and its parts
+        const float* part_o;
+        const float2* part_ml;
+    } prefix;
 };
 
 constexpr int kCUs = 256;
@@ -53,14 +68,9 @@ constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
 // and 111.  64 of 2000 and 4000, past the bound, would be faster whole: 30 and
 // 54, 55 and 68; of 8000 it is the same, 121.
 constexpr int kWholeTiles = 16;
-
-// the item that starts in share i and is cut at its end: its parts are in
-// slots 2 i + 1, 2 (i + 1), 2 (i + 2), ... of the workspace
-// (kPrefix, whose items are few: in the order of items, `h` its share)
-struct Cut {
-    int parts;  // 0: none
-    int b, block, h;
-};
+// Where all items are about as long, or only the device knows how long: up to
+// kAloneTiles, or up to four equal shares and kMoreTiles.
+constexpr int kAloneTiles = 36, kMoreTiles = 8;
 
 // The forms and the workgroups that a CU holds at once, by their registers and
 // LDS: O and Q are D R / 4 + D R / 8 registers a lane, and kKeys holds K and V

@@ -228,7 +228,7 @@ struct Sequence {
     bool poison;      // it has more than the table's
     int low, tiles;   // first key that any query sees (a multiple of 64), groups of 64 keys in the list
     int blocks;       // of rows
-    int prefix;       // kRest: keys that are not its own
+    int prefix, shared_by;  // kRest: keys that are not its own, and the group whose they are
     int first, last;  // kPrefix: its sequences
 };
 
@@ -253,7 +253,7 @@ __device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_att
         q.row0 = (int)seq_offset(a.offsets, sh.per, a.tokens, q.first);
         if (q.last > q.first && q.len > 0) q.n = max((int)seq_offset(a.offsets, sh.per, a.tokens, q.last) - q.row0, 0);
         q.tiles = max((q.len + 63) >> 6, 1);
-        q.blocks = (q.n * sh.group + sh.rows - 1) >> sh.log_rows;
+        q.blocks = (q.n * sh.group + (1 << sh.prefix.log_rows) - 1) >> sh.prefix.log_rows;
         return q;
     }
     q.row0 = (int)seq_offset(a.offsets, sh.per, a.tokens, b);
@@ -277,6 +277,7 @@ __device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_att
             else hi = mid - 1;
         }
         if (group_start(a, sh, g) <= b && b < group_start(a, sh, g + 1)) q.prefix = prefix_keys(c, a, sh, g);
+        q.shared_by = g;
         q.low = min(q.prefix, q.len) & ~63;
     }
     q.tiles = (q.len - q.low + 63) >> 6;
@@ -354,6 +355,7 @@ struct WorkList {
     bool by_item;
     int64_t w, upto;  // of the 64 sequences at hand: this lane's, and with those before
     int most = 0;     // kRest: this lane's longest item
+    int items = 0;    // and its items of the 64 sequences at hand
 
     __device__ __forceinline__ int count() const { return PART == kPrefix ? sh.groups : a.sequences; }
     __device__ __forceinline__ void take(int i) {
@@ -362,7 +364,10 @@ struct WorkList {
         if (b < count()) {
             const Sequence q = sequence<PART>(c, a, sh, b);
             w = (int64_t)q.blocks * c.kv_heads * (by_item ? 1 : q.tiles);
-            if (PART == kRest && q.blocks > 0) most = max(most, q.tiles);
+            if constexpr (PART == kRest) {
+                if (q.blocks > 0) most = max(most, q.tiles);
+                items = q.blocks * c.kv_heads;
+            }
         }
         upto = wave_scan(w);
     }
@@ -405,6 +410,7 @@ struct Item {
     int h;
     int all, block;  // rows of the sequence and key head, first row of the block
     int block_lo, block_hi, block_all_lo, block_all_hi;  // keys that any, and that all, rows of the block see
+    bool all_see, some_blind;  // kPrefix: every row but blind ones sees all keys; there are blind ones
 
     __device__ __forceinline__ Item(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_) : c(c_), a(a_), sh(sh_) {}
 
@@ -418,7 +424,7 @@ struct Item {
     __device__ __forceinline__ int upper(int tok) const {
         if constexpr (PART == kPrefix) {  // of its own sequence, as far as they are shared; 0: see `blind`
             int lo = seq.first, hi = seq.last - 1;
-            if (!a.offsets) lo = (int)((seq.row0 + tok) / sh.per);
+            if (!a.offsets) lo = (seq.row0 + tok) / sh.by_per;
             else
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
@@ -434,6 +440,34 @@ struct Item {
         const int len = min(max(a.lengths[b], 0), a.table_width * c.page_size);
         if (!a.causal) return len;
         return max(min(len - (int)seq_offset(a.offsets, sh.per, a.tokens, b + 1) + row + 1, len), 0);
+    }
+    // kRest: items of kPrefix that come before the group's
+    __device__ __forceinline__ int prefix_items() const {
+        int64_t blocks = 0;
+        for (int g = (int)(threadIdx.x & 63); g < seq.shared_by; g += 64) blocks += sequence<kPrefix>(c, a, sh, g).blocks;
+        return seq.shared_by ? (int)(from_lane(wave_scan(blocks), 63) * c.kv_heads) : 0;
+    }
+    // Where the shared keys' m, l and O of a row (token tok of the sequence, query
+    // head qh) are: in `parts` rows of the prefix's workspace, the first and those
+    // after it `step` apart; 0: one row of `carry`.
+    struct Carried {
+        int parts;
+        int64_t first, second, step;
+        __device__ __forceinline__ int64_t at(int p) const { return p == 0 ? first : second + (p - 1) * step; }
+    };
+    __device__ __forceinline__ Carried carried(int items, int tok, int qh) const {
+        const int64_t row = (int64_t)(seq.row0 + tok) * a.q_heads + qh;
+        if (sh.prefix.grid == 0) return {0, row, 0, 0};
+        const int start = (int)seq_offset(a.offsets, sh.per, a.tokens, group_start(a, sh, seq.shared_by));
+        const int end = (int)seq_offset(a.offsets, sh.per, a.tokens, group_start(a, sh, seq.shared_by + 1));
+        const int r = (seq.row0 + tok - start) * sh.group + qh - h * sh.group, rows = 1 << sh.prefix.log_rows;
+        const int64_t number = items + (int64_t)(r >> sh.prefix.log_rows) * c.kv_heads + h;
+        // (offsets that do not rise, or groups that overlap: any row there is)
+        if (seq.row0 + tok < start || seq.row0 + tok >= end || number >= sh.prefix.items) return {0, row, 0, 0};
+        const Cut cut = sh.prefix.cuts[number];
+        if (cut.parts == 0) return {0, row, 0, 0};
+        const int64_t slot = 2 * (int64_t)cut.h;  // cut.h: its share
+        return {cut.parts, (slot + 1) * rows + (r & (rows - 1)), (slot + 2) * rows + (r & (rows - 1)), 2 * (int64_t)rows};
     }
     // kSinks: of rows that see [.., top) the keys [0, sink_keys(top)) too
     __device__ __forceinline__ int sink_keys(int top) const { return PART == kSinks ? min(sh.sinks, top) : 0; }
@@ -463,27 +497,42 @@ struct Item {
         nan_left = false;
         if constexpr (PART == kPrefix) {
             // The shared pages stand in all its sequences' rows of the table; taken
-            // are those of the longest (an empty one may name none).  The least
-            // that a row sees, blind ones left out, bounds what all of the block's
-            // see: a sequence's first row, or 1 where that comes before its keys.
-            int64_t longest = -1;
-            int least = seq.len;
-            for (int s = seq.first + (int)(threadIdx.x & 63); s < seq.last; s += 64) {
+            // are those of the first that is long enough (an empty one may name
+            // none), or else of the longest.
+            int from = -1, long_one = 0, long_len = -1;
+            all_see = true;
+            some_blind = false;
+            for (int s0 = seq.first; s0 < seq.last; s0 += 64) {
+                const int s = min(s0 + (int)(threadIdx.x & 63), seq.last - 1);
                 const int row = (int)seq_offset(a.offsets, sh.per, a.tokens, s);
                 const int len = min(max(a.lengths[s], 0), a.table_width * c.page_size);
-                longest = max(longest, (int64_t)len << 32 | (uint32_t)(0x7fffffff - s));
-                if (len > 0 && (int)seq_offset(a.offsets, sh.per, a.tokens, s + 1) > row) least = min(least, max(seen_by(s, row), 1));
+                const bool rows = (int)seq_offset(a.offsets, sh.per, a.tokens, s + 1) > row;
+                const uint64_t fits = __ballot(len >= seq.len);
+                if (from < 0 && fits) from = min(s0 + (int)__builtin_ctzll(fits), seq.last - 1);
+                some_blind |= __any(len == 0 && rows);
+                all_see &= !__any(len > 0 && rows && seen_by(s, row) < seq.len);
+                if (from < 0 && len > long_len) {
+                    long_len = len;
+                    long_one = s;
+                }
             }
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                longest = max(longest, (int64_t)__shfl_xor((long long)longest, s));
-                least = min(least, __shfl_xor(least, s));
-            }
-            longest = uniform(longest);
-            table = a.page_table + (0x7fffffff - (int)(uint32_t)longest) * a.table_stride;
             block_lo = block_all_lo = 0;
-            block_hi = min((int)(longest >> 32), seq.len);
-            block_all_hi = uniform(least);
+            block_hi = block_all_hi = seq.len;
+            if (from < 0) {
+#pragma unroll
+                for (int s = 1; s < 64; s <<= 1) {
+                    const int len = __shfl_xor(long_len, s), one = __shfl_xor(long_one, s);
+                    if (len > long_len || (len == long_len && one < long_one)) {
+                        long_len = len;
+                        long_one = one;
+                    }
+                }
+                from = uniform(long_one);
+                block_hi = uniform(long_len);
+            }
+            table = a.page_table + from * a.table_stride;
+            // rows that see not all: what all rows of a block see is not looked for
+            if (!all_see) block_all_hi = 0;
             return;
         }
         table = a.page_table + b * a.table_stride;
@@ -615,10 +664,16 @@ struct Attend : Item<D, PART> {
             });
             if constexpr (S::REM) qv[r.value][S::KK - 1] = *(const x8*)(q + 64 * S::J + 8 * g);
             const int lo = this->lower(tok);
-            int hi = max(this->upper(tok), lo);
+            int hi = this->block_hi;
             if constexpr (PART == kPrefix) {
-                blind[r.value] = hi == 0;
-                if (hi == 0) hi = this->block_hi;
+                blind[r.value] = false;
+                if (!this->all_see || this->some_blind) {
+                    hi = this->upper(tok);
+                    blind[r.value] = hi == 0;
+                    if (hi == 0) hi = this->block_hi;
+                }
+            } else {
+                hi = max(this->upper(tok), lo);
             }
             low[r.value] = lo;
             top[r.value] = hi;
@@ -654,19 +709,39 @@ struct Attend : Item<D, PART> {
         });
     }
     // kRest: the shared keys' m, l and O, for the part of the item that has its
-    // first key
+    // first key.  KEYS: the waves take every fourth part, as of the keys.
     __device__ __forceinline__ void carry_in() {
-        if (KEYS && wave > 0) return;
+        constexpr int STRIDE = KEYS ? 4 : 1, U = 4;
+        const int items = this->prefix_items();
         const int j = here(this->j), g = here(this->g);
         static_for<0, R>([&](auto r) {
             const int row = row_of(r.value, j);
             if (row < all) {
                 const int tok = row / sh.by_group;
-                const int64_t at = (int64_t)(seq.row0 + tok) * a.q_heads + h * sh.group + row - tok * sh.group;
-                const float2 ml = sh.carry_ml[at];
-                m[r.value] = ml.x;
-                l[r.value] = g == 0 ? ml.y : 0.0f;  // (a lane's part of the sum)
-                static_for<0, S::N>([&](auto i) { o[r.value][i.value] = *(const f32x4*)(sh.carry_o + at * D + 16 * i.value + 4 * g); });
+                const auto from = this->carried(items, tok, h * sh.group + row - tok * sh.group);
+                const float* po = from.parts ? sh.prefix.part_o : sh.carry_o;
+                const float2* pml = from.parts ? sh.prefix.part_ml : sh.carry_ml;
+                const int parts = max(from.parts, 1);
+                for (int p0 = KEYS ? wave : 0; p0 < parts; p0 += U * STRIDE) {
+                    float2 ml[U];
+                    f32x4 w[U][S::N];
+                    static_for<0, U>([&](auto u) {  // (past the last: the last again, weighed 0)
+                        const int64_t at = from.at(min(p0 + u.value * STRIDE, parts - 1));
+                        ml[u.value] = pml[at];
+                        static_for<0, S::N>([&](auto i) { w[u.value][i.value] = *(const f32x4*)(po + at * D + 16 * i.value + 4 * g); });
+                    });
+                    float to = m[r.value];
+                    static_for<0, U>([&](auto u) { to = __builtin_fmaxf(to, ml[u.value].x); });
+                    const float shrink = __builtin_amdgcn_exp2f(m[r.value] - to);
+                    m[r.value] = to;
+                    l[r.value] *= shrink;
+                    static_for<0, S::N>([&](auto i) { o[r.value][i.value] *= shrink; });
+                    static_for<0, U>([&](auto u) {
+                        const float f = p0 + u.value * STRIDE < parts ? __builtin_amdgcn_exp2f(ml[u.value].x - to) : 0.0f;
+                        if (g == 0) l[r.value] += ml[u.value].y * f;  // (a lane's part of the sum)
+                        static_for<0, S::N>([&](auto i) { o[r.value][i.value] += w[u.value][i.value] * f; });
+                    });
+                }
             }
             large |= carried_large(m[r.value]);
         });
@@ -1085,19 +1160,27 @@ struct Tall : Item<D, PART> {
         const E* q = (const E*)a.q + (seq.row0 + tok) * a.q_strides[0] + qh * a.q_strides[1] + 8 * e;
         static_for<0, D / 16>([&](auto i) { qv[i.value] = *(const x8*)(q + 16 * i.value); });
         low = this->lower(tok);
-        top = max(this->upper(tok), low);
         if constexpr (PART == kPrefix) {
-            blind = top == 0;
-            if (blind) top = this->block_hi;
+            top = this->block_hi;
+            blind = false;
+            if (!this->all_see || this->some_blind) {
+                top = this->upper(tok);
+                blind = top == 0;
+                if (blind) top = this->block_hi;
+            }
+        } else {
+            top = max(this->upper(tok), low);
         }
         all_lo = any_lo = low;
         all_hi = any_hi = top;
+        if (PART != kPrefix || !this->all_see) {
 #pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            all_lo = max(all_lo, __shfl_xor(all_lo, s));
-            all_hi = min(all_hi, __shfl_xor(all_hi, s));
-            any_lo = min(any_lo, __shfl_xor(any_lo, s));
-            any_hi = max(any_hi, __shfl_xor(any_hi, s));
+            for (int s = 1; s < 32; s <<= 1) {
+                all_lo = max(all_lo, __shfl_xor(all_lo, s));
+                all_hi = min(all_hi, __shfl_xor(all_hi, s));
+                any_lo = min(any_lo, __shfl_xor(any_lo, s));
+                any_hi = max(any_hi, __shfl_xor(any_hi, s));
+            }
         }
         all_lo = uniform(all_lo);
         all_hi = uniform(all_hi);
@@ -1110,20 +1193,31 @@ struct Tall : Item<D, PART> {
         static_for<0, D / 16>([&](auto i) { loaded(qv[i.value]); });
     }
     __device__ __forceinline__ void carry_in() {
+        const int items = this->prefix_items();
         const int n = here(this->n), e = here(this->e);
         const int row = block + 32 * wave + n;
         if (row < all) {
             const int tok = row / sh.by_group;
-            const int64_t at = (int64_t)(seq.row0 + tok) * a.q_heads + h * sh.group + row - tok * sh.group;
-            const float2 ml = sh.carry_ml[at];
-            m = ml.x;
-            l = e == 0 ? ml.y : 0.0f;  // (a lane's part of the sum)
-            static_for<0, D / 32>([&](auto i) {
-                static_for<0, 4>([&](auto x) {
-                    const f32x4 w = *(const f32x4*)(sh.carry_o + at * D + 32 * i.value + 8 * x.value + 4 * e);
-                    static_for<0, 4>([&](auto z) { o[i.value][4 * x.value + z.value] = w[z.value]; });
+            const auto from = this->carried(items, tok, h * sh.group + row - tok * sh.group);
+            const float* po = from.parts ? sh.prefix.part_o : sh.carry_o;
+            const float2* pml = from.parts ? sh.prefix.part_ml : sh.carry_ml;
+            const int parts = max(from.parts, 1);
+            for (int p = 0; p < parts; ++p) {
+                const int64_t at = from.at(p);
+                const float2 ml = pml[at];
+                f32x4 w[D / 8];
+                static_for<0, D / 32>([&](auto i) {
+                    static_for<0, 4>([&](auto x) { w[4 * i.value + x.value] = *(const f32x4*)(po + at * D + 32 * i.value + 8 * x.value + 4 * e); });
                 });
-            });
+                const float to = __builtin_fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(ml.x - to), shrink = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l = l * shrink + (e == 0 ? ml.y * f : 0.0f);  // (a lane's part of the sum)
+                static_for<0, D / 32>([&](auto i) {
+                    static_for<0, 16>([&](auto x) {
+                        o[i.value][x.value] = o[i.value][x.value] * shrink + w[4 * i.value + x.value / 4][x.value % 4] * f;
+                    });
+                });
+            }
         }
         large |= carried_large(m);
     }
@@ -1424,19 +1518,24 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
     if (!whole) {
         total = list.total();
         if constexpr (PART == kRest) {
-            // how long items are only the device knows: one workgroup an item then
-            // too, none cut (attend_launch has workgroups enough for that)
+            // how long items are only the device knows (attend_launch has workgroups
+            // enough for one an item)
             int most = list.most;
 #pragma unroll
             for (int s = 1; s < 64; s <<= 1) most = max(most, __shfl_xor(most, s));
-            whole = uniform(most) <= sh.whole_tiles;
+            const int64_t even = quotient(total + sh.grid - 1, sh.grid);
+            whole = uniform(most) <= max(sh.whole_tiles, 4 * (int)even + sh.whole_more);
             if (whole && (int)blockIdx.x < sh.grid && threadIdx.x == 0) cuts[blockIdx.x].parts = 0;
             list.by_item = whole;
+            if (whole) {
+                list.w = list.items;
+                list.upto = wave_scan(list.w);
+            }
             if (!whole && (int)blockIdx.x >= sh.grid) return;
         }
     }
     if (whole) {
-        b = list.find(blockIdx.x, before, false);
+        b = list.find(blockIdx.x, before, PART == kRest && sh.grid && list.count() <= 64);
         if (b < 0) {
             if constexpr (PART != kPrefix) {
                 if (sh.grid == 0) clear_rest<E, D>(a, blockIdx.x - before, gridDim.x - before);
@@ -1464,9 +1563,11 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
     // kPrefix: which of all items this is, whose cut is cuts[] of that
     int64_t number = 0;
     if constexpr (PART == kPrefix) {
-        if (sh.grid) {
-            for (int g = (int)(threadIdx.x & 63); g < b; g += 64) number += sequence<PART>(c, a, sh, g).blocks;
-            number = from_lane(wave_scan(number), 63) * c.kv_heads + item;
+        number = item;
+        if (sh.grid && b > 0) {
+            int64_t blocks = 0;
+            for (int g = (int)(threadIdx.x & 63); g < b; g += 64) blocks += sequence<PART>(c, a, sh, g).blocks;
+            number += from_lane(wave_scan(blocks), 63) * c.kv_heads;
         }
     }
     Cut cut{0, 0, 0, 0};
@@ -1480,13 +1581,13 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
         w.run(tile, upto);
         if (tile == 0 && upto == w.seq.tiles) {
             w.store();
-            if (PART == kPrefix && sh.grid && threadIdx.x == 0 && number < sh.items) cuts[number].parts = 0;
+            if (PART == kPrefix && sh.grid && threadIdx.x == 0 && number < sh.prefix.items) cuts[number].parts = 0;
         } else {
             w.store_part(2 * (int)blockIdx.x + (tile == 0 ? 1 : 0), part_o, part_ml);
             if (tile == 0) {  // its last group lies `past` groups past this share's end
                 const int past = (int)(at + w.seq.tiles - 1 - stop);
                 cut = {share > past ? 2 : past / (int)share + 2, b, block, PART == kPrefix ? (int)blockIdx.x : h};
-                if (PART == kPrefix && threadIdx.x == 0 && number < sh.items) cuts[number] = cut;
+                if (PART == kPrefix && threadIdx.x == 0 && number < sh.prefix.items) cuts[number] = cut;
             }
         }
         at += upto - tile;
@@ -1511,25 +1612,17 @@ __global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_arg
                                                    const float2* part_ml, const Cut* cuts) {
     constexpr int C = (D + 63) / 64;
     const int groups = (sh.live + sh.join_rows - 1) / sh.join_rows;
-    int share = blockIdx.x / groups;
-    int64_t before = 0;
-    if constexpr (PART == kPrefix) {  // an item's number
-        if (WorkList<PART>{c, a, sh, true, 0, 0}.find(share, before, false) < 0) return;
-    } else if (share >= sh.grid) {
+    const int share = blockIdx.x / groups;
+    if (share >= sh.grid) {
         clear_rest<E, D>(a, blockIdx.x - sh.grid * groups, gridDim.x - sh.grid * groups);
         return;
     }
-    Cut cut = cuts[share];
+    const Cut cut = cuts[share];
     if (cut.parts == 0) return;
-    if constexpr (PART == kPrefix) {
-        const int item = (int)(share - before);
-        share = cut.h;
-        cut.h = item - item / sh.by_heads * c.kv_heads;
-    }
     const Sequence seq = sequence<PART>(c, a, sh, cut.b);
     const int block = cut.block * sh.rows, all = seq.n * sh.group;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool wide = PART != kPrefix && cut.parts > 8;
+    const bool wide = cut.parts > 8;
     const int first = (int)(blockIdx.x % groups) * sh.join_rows;
     const int end = min(min(first + sh.join_rows, sh.live), all - block);
     __shared__ float sl[4], so[4][64 * C];
@@ -1566,14 +1659,6 @@ __global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_arg
         const int place = (block + row) / sh.by_group;
         const int64_t tok = seq.row0 + place;
         const int qh = cut.h * sh.group + block + row - place * sh.group;
-        if constexpr (PART == kPrefix) {
-            const int64_t at = tok * a.q_heads + qh;
-#pragma unroll
-            for (int x = 0; x < C; ++x)
-                if (D % 64 == 0 || lane + 64 * x < D) sh.carry_o[at * D + lane + 64 * x] = o[x];
-            if (lane == 0) sh.carry_ml[at] = make_float2(m, l);
-            continue;
-        }
         E* y = (E*)a.out + tok * a.out_strides[0] + qh * a.out_strides[1];
 #pragma unroll
         for (int x = 0; x < C; ++x)
@@ -1597,9 +1682,11 @@ void launch_dim(const mfft_cache& c, const mfft_attend_args& a, const AttendLaun
         else if constexpr (D <= 96) attend_kernel<E, D, kKeys4, PART><<<grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
     }
     mark(s);
-    if (w.sh.grid) {
-        join_kernel<E, D, PART><<<(uint32_t)w.join_grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
-        mark(s);
+    if constexpr (PART != kPrefix) {
+        if (w.sh.grid) {
+            join_kernel<E, D, PART><<<(uint32_t)w.join_grid, 256, 0, s>>>(c, a, w.sh, po, ml, cuts);
+            mark(s);
+        }
     }
 }
 

@@ -47,6 +47,7 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     w.sh.least = w.sh.rows / 4 > kLeastTiles ? w.sh.rows / 4 : kLeastTiles;
     if (part == kPrefix) w.sh.least = kLeastTiles;
     w.sh.log_rows = ilog2(w.sh.rows);
+    w.sh.by_per = divisor((uint32_t)w.sh.per);
     w.sh.by_group = divisor(w.sh.group);
     w.sh.by_heads = divisor(c.kv_heads);
     w.sh.live = !a.offsets && part != kPrefix && rows < w.sh.rows ? (int)rows : w.sh.rows;
@@ -57,28 +58,34 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     w.sh.block_tokens = (w.sh.rows - 1) / w.sh.group + 2;
     if (part == kSinks && a.causal)
         longest = std::min(longest, ((o.sinks + 63) & ~(int64_t)63) + a.window + std::min<int64_t>(w.sh.block_tokens, a.tokens) + 126);
-    const int64_t each = std::max<int64_t>(1, std::max<int64_t>(sequences, a.tokens * w.sh.group / w.sh.rows) * c.kv_heads / at_once);
-    const bool whole = longest <= 64 * kWholeTiles * each;
+    const int64_t each_items = std::max<int64_t>(sequences, a.tokens * w.sh.group / w.sh.rows) * c.kv_heads;
+    const int64_t each = std::max<int64_t>(1, each_items / at_once);
+    bool whole = longest <= 64 * kWholeTiles * each;
+    if (part == kSinks && a.causal) {
+        const int64_t tiles = (longest + 63) / 64, even = each_items * tiles / at_once;
+        whole = tiles <= std::max<int64_t>(kAloneTiles, 4 * even + kMoreTiles);
+    }
     w.idle = a.offsets && part != kPrefix ? kIdle : 0;
     w.grid = items + w.idle;
+    w.sh.prefix.log_rows = w.sh.log_rows;
+    w.sh.prefix.items = items;
     if (!whole) {
         // as many shares as workgroups run at once
         w.sh.grid = (int)at_once;
+        w.sh.prefix.grid = w.sh.grid;
         w.grid = w.sh.grid;
         if (part == kRest) {
-            w.sh.whole_tiles = (int)std::min<int64_t>(kWholeTiles * each, 1 << 20);
+            w.sh.whole_tiles = kAloneTiles;
+            w.sh.whole_more = kMoreTiles;
             w.grid = std::max<int64_t>(w.grid, items);
         }
         // few sequences and heads: their items are cut into many parts
         w.sh.join_rows = w.sh.live <= 16 && w.sh.grid >= 8 * (int64_t)sequences * c.kv_heads ? 1 : w.sh.live > 16 ? 8 : 4;
         w.o_bytes = (int64_t)2 * w.sh.grid * w.sh.rows * D * 4;
         w.ml_bytes = (int64_t)2 * w.sh.grid * w.sh.rows * 8;
-        // kPrefix: items, few and long, by number (more than `items` only in groups
-        // that overlap, which are none)
-        if (part == kPrefix) w.sh.join_rows = 4;
-        w.sh.items = part == kPrefix ? items : w.sh.grid;
-        w.cut_bytes = w.sh.items * (int64_t)sizeof(Cut);
-        w.join_grid = w.sh.items * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows) + w.idle;
+        // (more items than `items` there are only of groups that overlap, which are none)
+        w.cut_bytes = (part == kPrefix ? items : w.sh.grid) * (int64_t)sizeof(Cut);
+        if (part != kPrefix) w.join_grid = (int64_t)w.sh.grid * ((w.sh.live + w.sh.join_rows - 1) / w.sh.join_rows) + w.idle;
     }
     return w;
 }
@@ -89,11 +96,10 @@ int64_t part_bytes(const AttendLaunch& w) { return (w.o_bytes + w.ml_bytes + w.c
 
 bool attend_supported(int head_dim) { return head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256; }
 
-// The parts' own, which may be the same memory as they run one after the other,
-// then what the prefix leaves for each row.
+// kPrefix's, kRest's, then what the former leaves for each row.
 int64_t attend_workspace(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o) {
     if (with_prefix(a, o))
-        return std::max(part_bytes(attend_launch(c, a, o, kPrefix)), part_bytes(attend_launch(c, a, o, kRest))) +
+        return part_bytes(attend_launch(c, a, o, kPrefix)) + part_bytes(attend_launch(c, a, o, kRest)) +
                a.tokens * a.q_heads * (4 * c.head_dim + 8);
     const AttendLaunch w = attend_launch(c, a, o, with_sinks(a, o) ? kSinks : kAll);
     return w.o_bytes + w.ml_bytes + w.cut_bytes;
@@ -110,10 +116,17 @@ bool attend_launch_fits(const mfft_cache& c, const mfft_attend_args& a, const mf
 hipError_t launch_attend(const mfft_cache& c, const mfft_attend_args& a, const mfft_attend_options& o, hipStream_t stream) {
     if (with_prefix(a, o)) {
         AttendLaunch p = attend_launch(c, a, o, kPrefix), r = attend_launch(c, a, o, kRest);
-        p.sh.carry_o = r.sh.carry_o = (float*)((char*)a.workspace + std::max(part_bytes(p), part_bytes(r)));
+        char* const ws = (char*)a.workspace;
+        p.sh.carry_o = r.sh.carry_o = (float*)(ws + part_bytes(p) + part_bytes(r));
         p.sh.carry_ml = r.sh.carry_ml = (float2*)(r.sh.carry_o + a.tokens * a.q_heads * c.head_dim);
+        r.sh.prefix = p.sh.prefix;
+        r.sh.prefix.part_o = (const float*)ws;
+        r.sh.prefix.part_ml = (const float2*)(ws + p.o_bytes);
+        r.sh.prefix.cuts = (const Cut*)(ws + p.o_bytes + p.ml_bytes);
         launch_part<kPrefix>(c, a, p, stream);
-        launch_part<kRest>(c, a, r, stream);
+        mfft_attend_args rest = a;
+        rest.workspace = ws + part_bytes(p);
+        launch_part<kRest>(c, rest, r, stream);
     } else if (with_sinks(a, o)) {
         launch_part<kSinks>(c, a, attend_launch(c, a, o, kSinks), stream);
     } else {
