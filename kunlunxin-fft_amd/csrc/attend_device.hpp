@@ -30,8 +30,8 @@
 //
 // Bound: for few rows the codes' bytes (one token over 2^18 tokens of 8 heads
 // of 128, 537 MB: 99 us, 5.4 TB/s), for many the products and, not overlapped
-// with them, the softmax (2048 tokens of 32 heads over 32768: 1.23 ms, 870
-// TFLOP/s, in float16 1.31 ms; the products alone 732 us).
+// with them, the softmax (2048 tokens of 32 heads over 32768: 1.18 ms, 910
+// TFLOP/s; the products alone 732 us).
 #pragma once
 
 #include <algorithm>
@@ -1329,6 +1329,28 @@ struct Tall : Item<D, PART> {
         });
     }
 
+    // N products, each with an operand from LDS: kAhead loads are under way while as
+    // many products are made.  Left alone the compiler puts each load right before
+    // its product, which then waits for it: 2048 tokens of 32 heads over 32768 took
+    // 1241 us instead of 1179, the case of sinks above 189 instead of 178.  Eight
+    // ahead need more registers than two workgroups a CU have.
+    static constexpr int kAhead = 4;
+    template <int N, class At, class Use>
+    static __device__ __forceinline__ void products(At at, Use use) {
+        static_assert(N % kAhead == 0);
+        x8 f[2][kAhead];
+        static_for<0, kAhead>([&](auto x) { f[0][x.value] = *(const x8*)at(x); });
+        static_for<0, N / kAhead>([&](auto b) {
+            if constexpr (b.value + 1 < N / kAhead)
+                static_for<0, kAhead>([&](auto x) {
+                    f[(b.value + 1) % 2][x.value] = *(const x8*)at(std::integral_constant<int, (b.value + 1) * kAhead + x.value>{});
+                });
+            __builtin_amdgcn_sched_barrier(0);
+            static_for<0, kAhead>([&](auto x) { use(std::integral_constant<int, b.value * kAhead + x.value>{}, f[b.value % 2][x.value]); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+
     __device__ __forceinline__ void run(int tile, int upto) {
         int from, end;
         this->span(tile, upto, from, end);
@@ -1379,19 +1401,22 @@ struct Tall : Item<D, PART> {
                 const uint8_t* kb = lds.k[buf] + k_at;
                 static_for<0, 2>([&](auto t) {
                     static_for<0, 16>([&](auto x) { s[t.value][x.value] = 0.0f; });
-                    static_for<0, D / 16>([&](auto i) {
-                        const x8 k = *(const x8*)(kb + t.value * (32 * KROW + 256) + 32 * i.value);
-                        s[t.value] = M::mfma(k, qv[i.value], s[t.value]);
-                    });
                 });
+                products<2 * D / 16>(
+                    [&](auto x) { return kb + (x.value % 2) * (32 * KROW + 256) + 32 * (x.value / 2); },
+                    [&](auto x, x8 k) { s[x.value % 2] = M::mfma(k, qv[x.value / 2], s[x.value % 2]); });
                 weights(s, p, key0 < all_lo || key0 + 64 > all_hi, key0);
                 const uint8_t* vb = lds.v[buf] + v_at;
-                static_for<0, D / 32>([&](auto i) {
-                    static_for<0, 4>([&](auto x) {  // product x: keys 32 (x / 2) + 16 e + 8 (x % 2) and on
-                        const x8 v = *(const x8*)(vb + (((x.value % 2) * 4 + 2 * (x.value / 2)) * D + 32 * i.value) * 16);
-                        o[i.value] = M::mfma(v, p[x.value], o[i.value]);
+                // product x of a block of channels: keys 32 (x / 2) + 16 e + 8 (x % 2) and on
+                products<4 * D / 32>(
+                    [&](auto z) {
+                        constexpr int i = z.value % (D / 32), x = z.value / (D / 32);
+                        return vb + (((x % 2) * 4 + 2 * (x / 2)) * D + 32 * i) * 16;
+                    },
+                    [&](auto z, x8 v) {
+                        constexpr int i = z.value % (D / 32), x = z.value / (D / 32);
+                        o[i] = M::mfma(v, p[x], o[i]);
                     });
-                });
             }
             buf ^= 1;
             if (more) stash(buf, this->key_at(place + 64));
