@@ -2,6 +2,7 @@
 // call makes, and their shapes.  The kernels are in attend_device.hpp, compiled
 // for each part of the keys in a file of its own.
 #include <algorithm>
+#include <cmath>
 
 #include "attend.hpp"
 #include "mfft_device.hpp"
@@ -45,7 +46,6 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     // a cut costs its rows' partial sums, written and read again: about a
     // quarter as many groups of keys as it has rows
     w.sh.least = w.sh.rows / 4 > kLeastTiles ? w.sh.rows / 4 : kLeastTiles;
-    if (part == kPrefix) w.sh.least = kLeastTiles;
     w.sh.log_rows = ilog2(w.sh.rows);
     w.sh.by_per = divisor((uint32_t)w.sh.per);
     w.sh.by_group = divisor(w.sh.group);
@@ -64,6 +64,18 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     if (part == kSinks && a.causal) {
         const int64_t tiles = (longest + 63) / 64, even = each_items * tiles / at_once;
         whole = tiles <= std::max<int64_t>(kAloneTiles, 4 * even + kMoreTiles);
+    }
+    if (part == kPrefix) {
+        // Its cuts cost no launch, so that items are cut as soon as workgroups are
+        // left (134 sequences of 8 heads of 256 in 7 groups of 701 shared tokens 53 us
+        // instead of 63).  But each sequence's launch reads all parts of its group's
+        // item, sixteen at a time: of T groups of keys about 2 sqrt(T), and 4 sqrt(T)
+        // of the forms that take longer over a group (shares of four groups
+        // and of this many, in us: 4 sequences in 2 groups of 26241 tokens 45 and 37, 3 of
+        // 96024 each alone 52 and 45; 8 of 32768 together the same, 40).
+        if (each_items < at_once) whole = longest <= 64 * kLeastTiles;
+        const double root = std::sqrt((double)longest / 64.0);
+        w.sh.least = std::max(kLeastTiles, (int)(w.form == kKeys1 || w.form == kKeys2 ? root / 2 : root / 4));
     }
     w.idle = a.offsets && part != kPrefix ? kIdle : 0;
     w.grid = items + w.idle;

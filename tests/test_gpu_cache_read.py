@@ -6,7 +6,7 @@ import torch
 
 import lm_more_oracle as more
 import lm_oracle as lm
-from kunlunxin_fft_amd import PagedCache, append_paged_cache, read_paged_cache
+from kunlunxin_fft_amd import PagedCache, append_paged_cache, native, read_paged_cache
 from test_gpu_paged_cache import _f64, _i32, _randn, _table
 
 pytestmark = pytest.mark.gpu
@@ -155,3 +155,23 @@ def test_side_stream_and_graph(gpu):
         for a, b in zip((k, v), read_paged_cache(cache, table, starts, 160)):
             assert torch.equal(a.view(torch.int16), b.view(torch.int16))  # bits: some are NaN
     del graph
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_outputs_with_strides(gpu, dtype):
+    """The C entry's outputs may lie in larger tensors: what is between stays."""
+    counts, page, heads, dim = [20, 3, 41], 32, 3, 64
+    table, pool = _table([9 + n for n in counts], page, gpu, 11)
+    cache = _random(gpu, pool, heads, dim, page, 12)
+    t, off, starts = sum(counts), _i32(lm.offsets_of(counts), gpu), _i32([9, 0, 5], gpu)
+    fused = torch.full((t, 2 * heads + 1, dim + 16), 7.0, dtype=lm.DTYPES[dtype], device=gpu)
+    by_head = torch.full((heads, t + 2, dim), 7.0, dtype=lm.DTYPES[dtype], device=gpu)
+    k, v = fused[:, 2:2 + heads, 8:8 + dim], by_head[:, 1:1 + t].transpose(0, 1)
+    args = native.READ_ARGS.pack(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], table.data_ptr(), starts.data_ptr(),
+                                 off.data_ptr(), table.stride(0), t, table.shape[1], len(counts), getattr(native, dtype.replace("fp", "F").replace("bf", "BF")))
+    native.cache_read(cache._packed, args, torch.cuda.current_stream(gpu).cuda_stream)
+    for got, want in zip((k, v), read_paged_cache(cache, table, starts, t, offsets=off, dtype=lm.DTYPES[dtype])):
+        np.testing.assert_array_equal(_f64(got), _f64(want))
+    keep = torch.ones_like(fused, dtype=torch.bool)
+    keep[:, 2:2 + heads, 8:8 + dim] = False
+    assert bool((fused[keep] == 7).all()) and bool((by_head[:, [0, -1]] == 7).all())

@@ -128,3 +128,30 @@ def test_a_captured_loop(gpu):
         lengths += 1
         after += 1
     del graph
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that are cut over the chip, on two streams with nothing to order
+    them: each with a workspace of its own, and the same bits as alone."""
+    heads, hq, dim, page, batch, shared = 2, 8, 64, 16, 4, 600
+    own = 40
+    pool = shared + batch * own
+    cache = PagedCache.empty(pool, heads, dim, page, gpu)
+    every = torch.arange(pool, dtype=torch.int32, device=gpu)
+    k, v = (_randn((pool * page, heads, dim), "bf16", gpu, s) for s in (1, 2))
+    append_paged_cache(cache, k, v, every[None], _i32([0], gpu), offsets=_i32([0, pool * page], gpu))
+    table = torch.cat([every[:shared].expand(batch, shared), every[shared:].view(batch, own)], 1).contiguous()
+    q = [_randn((batch, hq, dim), "bf16", gpu, s) for s in (3, 4)]
+    lengths = _i32([shared * page + 300 + 90 * b for b in range(batch)], gpu)
+    kinds = [dict(prefix_pages=_i32([shared], gpu)), dict(window=7000, sinks=100)]
+    alone = [[attend_paged_cache(cache, x, table, lengths, **kw) for kw in kinds] for x in q]
+    streams = [torch.cuda.Stream(gpu) for _ in q]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] += [attend_paged_cache(cache, q[i], table, lengths, **kw) for kw in kinds]
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, alone[i][n % 2]) for n, y in enumerate(got[i]))
