@@ -6,13 +6,12 @@
 // of 128 channels, 134 MB: 29 us, 4.6 TB/s (a pair a thread: 73 us); float32,
 // 100003 tokens of 8 heads of 96, 614 MB: 111 us, 5.5 TB/s (209 us).
 #include <algorithm>
+#include <type_traits>
 
 #include "lm_device.hpp"
 
 namespace mfft {
 namespace {
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // One thread per (token, head, pair), any strides, alignment and sizes.
 template <class E>
@@ -116,14 +115,19 @@ __global__ __launch_bounds__(256) void rotary_chunk_kernel(RotaryTables t, mfft_
 // their own: the workgroup makes its tokens' roots together.  Roots loaded by
 // each thread as above: 1024 tokens of 40 heads of 128 21 us, so 9.3 (plain
 // positions 7.5, and 9.3 made together, as they take one more round of loads);
-// 50001 of 16 heads of 64 in float32 97 and 85 us (4.8 TB/s).
-template <class E, bool HALF>
+// 50001 of 16 heads of 64 in float32 97 and 85 us (4.8 TB/s).  V is 16 bytes of
+// elements, or 4 (8 where neighbours are pairs or E is float) where pairs,
+// strides or addresses keep no more: 2142 tokens of 49 heads of 128 of which 20
+// channels are turned, 14.9 us, neighbouring pairs 12.4 (a pair a thread: 30.7).
+template <class E, bool HALF, int V>
 __global__ __launch_bounds__(256) void rotary_axes_kernel(RotaryTables t, mfft_rotary_args a, int64_t axis_stride,
                                                            int chunks, int tokens, Divisor by_pairs, int heads) {
-    constexpr int V = 16 / sizeof(E), C = HALF ? V : V / 2;  // elements of a load, pairs of a chunk
+    constexpr int C = HALF ? V : V / 2;  // V: elements of a load; pairs of a chunk
+    typedef uint32_t Words __attribute__((ext_vector_type(V * sizeof(E) / 4)));
+    typedef typename std::conditional<V * sizeof(E) == 4, uint32_t, Words>::type Held;
     union Vec {
         E e[V];
-        u32x4 w;
+        Held w;
     };
     __shared__ float4 ws[C / 2 * 256];
     // tokens of all batches, one after the other: this workgroup's first, how many
@@ -210,13 +214,12 @@ __global__ __launch_bounds__(256) void rotary_axes_kernel(RotaryTables t, mfft_r
     }
 }
 
-// Whether every load and store of rotary_chunk_kernel is 16-byte aligned.
-bool chunked(const RotaryTables& t, const mfft_rotary_args& a) {
-    const int v = a.dtype == MFFT_F32 ? 4 : 8;
+// Whether chunks hold whole loads of v elements, each of them aligned.
+bool chunked(const RotaryTables& t, const mfft_rotary_args& a, int v) {
     const bool half = t.layout == MFFT_ROTARY_HALF;
     if (t.pairs % (half ? v : v / 2) || a.head_dim % (half ? 2 * v : v)) return false;
     if (t.axes > 1 && a.head_dim / (half ? 2 * v : v) > 256) return false;  // a workgroup has whole tokens
-    if (((uintptr_t)a.in | (uintptr_t)a.out) & 15) return false;
+    if (((uintptr_t)a.in | (uintptr_t)a.out) & (v * (a.dtype == MFFT_F32 ? 4 : 2) - 1)) return false;
     for (int i = 0; i < 3; ++i)
         if (a.in_strides[i] % v || a.out_strides[i] % v) return false;
     return true;
@@ -230,31 +233,39 @@ int heads_a_thread(int64_t threads, int heads) {
     return slabs >= heads ? least : std::max((int)((heads + slabs - 1) / slabs), least);
 }
 
+template <class E, bool HALF, int V>
+void launch_axes(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_stride, hipStream_t s) {
+    const int chunks = a.head_dim / (HALF ? 2 * V : V), tokens = 256 / chunks;
+    const int64_t all = a.batch * a.tokens;
+    const int heads = heads_a_thread(all * chunks, a.heads);
+    const dim3 grid((uint32_t)((all + tokens - 1) / tokens), (uint32_t)((a.heads + heads - 1) / heads));
+    rotary_axes_kernel<E, HALF, V><<<grid, 256, 0, s>>>(t, a, axis_stride, chunks, tokens, divisor(t.pairs), heads);
+}
+
 template <class E>
 void launch_type(const RotaryTables& t, const mfft_rotary_args& a, int64_t axis_stride, hipStream_t s) {
-    if (chunked(t, a)) {
-        const bool half = t.layout == MFFT_ROTARY_HALF;
-        const uint32_t chunks = (uint32_t)(a.head_dim * sizeof(E) / (half ? 32 : 16));
+    constexpr int V = 16 / sizeof(E);
+    const bool half = t.layout == MFFT_ROTARY_HALF;
+    if (t.axes > 1) {
+        if (half && chunked(t, a, V)) return launch_axes<E, true, V>(t, a, axis_stride, s);
+        if (half && chunked(t, a, 2)) return launch_axes<E, true, 2>(t, a, axis_stride, s);
+        if (!half && chunked(t, a, V)) return launch_axes<E, false, V>(t, a, axis_stride, s);
+        if constexpr (V > 4)
+            if (!half && chunked(t, a, 4)) return launch_axes<E, false, 4>(t, a, axis_stride, s);
+    } else if (chunked(t, a, V)) {
+        const uint32_t chunks = (uint32_t)(a.head_dim / (half ? 2 * V : V));
         const uint32_t total = (uint32_t)(a.batch * a.tokens) * chunks;
         const int heads = heads_a_thread(total, a.heads);
         const uint32_t slabs = (uint32_t)((a.heads + heads - 1) / heads);
-        if (t.axes > 1) {
-            const int64_t all = a.batch * a.tokens, tokens = 256 / chunks;
-            const dim3 grid((uint32_t)((all + tokens - 1) / tokens), slabs);
-            const Divisor by = divisor(t.pairs);
-            if (half) rotary_axes_kernel<E, true><<<grid, 256, 0, s>>>(t, a, axis_stride, (int)chunks, (int)tokens, by, heads);
-            else rotary_axes_kernel<E, false><<<grid, 256, 0, s>>>(t, a, axis_stride, (int)chunks, (int)tokens, by, heads);
-            return;
-        }
         const dim3 grid((uint32_t)(((uint64_t)total + 255) / 256), slabs);
         if (half) rotary_chunk_kernel<E, true><<<grid, 256, 0, s>>>(t, a, chunks, total, heads);
         else rotary_chunk_kernel<E, false><<<grid, 256, 0, s>>>(t, a, chunks, total, heads);
         return;
     }
-    const uint32_t half = (uint32_t)a.head_dim / 2;
-    const uint32_t total = (uint32_t)(a.batch * a.tokens * a.heads) * half;
+    const uint32_t pairs = (uint32_t)a.head_dim / 2;
+    const uint32_t total = (uint32_t)(a.batch * a.tokens * a.heads) * pairs;
     const uint32_t grid = (uint32_t)(((uint64_t)total + 255) / 256);
-    rotary_pair_kernel<E><<<grid, 256, 0, s>>>(t, a, axis_stride, half, total);
+    rotary_pair_kernel<E><<<grid, 256, 0, s>>>(t, a, axis_stride, pairs, total);
 }
 
 }  // namespace
