@@ -69,13 +69,14 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
         // Its cuts cost no launch, so that items are cut as soon as workgroups are
         // left (134 sequences of 8 heads of 256 in 7 groups of 701 shared tokens 53 us
         // instead of 63).  But each sequence's launch reads all parts of its group's
-        // item, sixteen at a time: of T groups of keys about 2 sqrt(T), and 4 sqrt(T)
-        // of the forms that take longer over a group (shares of four groups
-        // and of this many, in us: 4 sequences in 2 groups of 26241 tokens 45 and 37, 3 of
-        // 96024 each alone 52 and 45; 8 of 32768 together the same, 40).
+        // item: of T groups of keys about 2 sqrt(T) (shares of four groups at least,
+        // of half and of the whole root, in us: 4 sequences in 2 groups of 26241
+        // tokens 45, 37 and 39, 24 of 65536 together 76, 63 and 83, 8 tokens of 3
+        // heads of 256 over 57908 483, 204 and 187; 8 sequences of 32768 together 40,
+        // 40 and 47).
         if (each_items < at_once) whole = longest <= 64 * kLeastTiles;
         const double root = std::sqrt((double)longest / 64.0);
-        w.sh.least = std::max(kLeastTiles, (int)(w.form == kKeys1 || w.form == kKeys2 ? root / 2 : root / 4));
+        w.sh.least = std::max(kLeastTiles, (int)(root / 2));
     }
     w.idle = a.offsets && part != kPrefix ? kIdle : 0;
     w.grid = items + w.idle;
