@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "mfft_internal.hpp"
 
 namespace mfft {
@@ -29,7 +31,7 @@ struct Cut {
 
 struct AttendShape {
     int group;        // query heads a key head
-    Divisor by_group, by_heads, by_per;
+    Divisor by_group, by_heads;
     int rows, log_rows;  // rows of a block, a power of two
     int units;        // page_size / 16
     uint64_t magic;   // floor(2^32 / units) + 1: x / units = x * magic >> 32, exact for x < 2^26
@@ -37,9 +39,16 @@ struct AttendShape {
     int least;        // fewest groups of 64 keys in a share
     int live;         // rows of a block that can be in use
     int join_rows;    // rows of a workgroup of the join
+    int64_t per;      // queries of each sequence without offsets
+};
+// What the other parts' kernels need too.  kAll's are not given it: arguments
+// that they do not use, between and before those that they do, are more and
+// smaller loads of arguments, each waited for, wherever an item begins (117
+// sequences of 4 keys of 4 heads of 256 20.6 us instead of 19.7).
+struct PartShape : AttendShape {
+    Divisor by_per;
     int whole_tiles, whole_more;  // kRest: see kAloneTiles
     int block_tokens; // kSinks: tokens of a sequence whose rows a block can have
-    int64_t per;      // queries of each sequence without offsets
     // kSinks
     int sinks;        // keys that stay visible
     // kPrefix, kRest
@@ -56,6 +65,8 @@ struct AttendShape {
         const float2* part_ml;
     } prefix;
 };
+template <Part PART>
+using ShapeOf = typename std::conditional<PART == kAll, AttendShape, PartShape>::type;
 
 constexpr int kCUs = 256;
 constexpr int kLeastTiles = 4;  // one group of 64 keys a wave
@@ -93,7 +104,7 @@ constexpr int attend_per_cu(int d, Form f) {
 constexpr int kIdle = 32;
 
 struct AttendLaunch {
-    AttendShape sh;
+    PartShape sh;
     Form form;
     int64_t grid, join_grid, o_bytes, ml_bytes, cut_bytes;
     int idle;  // workgroups more than work, see clear_rest: of the join where there is one

@@ -248,10 +248,10 @@ struct Sequence {
 };
 
 // Keys that group g of sequences shares: whole pages.
-__device__ __forceinline__ int prefix_keys(const mfft_cache& c, const mfft_attend_args& a, const AttendShape& sh, int g) {
+__device__ __forceinline__ int prefix_keys(const mfft_cache& c, const mfft_attend_args& a, const PartShape& sh, int g) {
     return min(max(sh.prefix_pages[g], 0), a.table_width) * c.page_size;
 }
-__device__ __forceinline__ int group_start(const mfft_attend_args& a, const AttendShape& sh, int g) {
+__device__ __forceinline__ int group_start(const mfft_attend_args& a, const PartShape& sh, int g) {
     const int b = sh.prefix_groups ? sh.prefix_groups[g] : g * a.sequences;
     return min(max(b, 0), a.sequences);
 }
@@ -259,7 +259,7 @@ __device__ __forceinline__ int group_start(const mfft_attend_args& a, const Atte
 // kPrefix: group b as the kernels take a sequence: its rows are all its
 // sequences' rows, its keys the shared ones.
 template <Part PART>
-__device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_attend_args& a, const AttendShape& sh, int b) {
+__device__ __forceinline__ Sequence sequence(const mfft_cache& c, const mfft_attend_args& a, const ShapeOf<PART>& sh, int b) {
     Sequence q{};
     if constexpr (PART == kPrefix) {
         q.first = group_start(a, sh, b);
@@ -366,13 +366,16 @@ template <Part PART>
 struct WorkList {
     const mfft_cache& c;
     const mfft_attend_args& a;
-    const AttendShape& sh;
+    const ShapeOf<PART>& sh;
     bool by_item;
     int64_t w, upto;  // of the 64 sequences at hand: this lane's, and with those before
     int most = 0;     // kRest: this lane's longest item
     int items = 0;    // and its items of the 64 sequences at hand
 
-    __device__ __forceinline__ int count() const { return PART == kPrefix ? sh.groups : a.sequences; }
+    __device__ __forceinline__ int count() const {
+        if constexpr (PART == kPrefix) return sh.groups;
+        return a.sequences;
+    }
     __device__ __forceinline__ void take(int i) {
         const int b = i + (int)(threadIdx.x & 63);
         w = 0;
@@ -419,7 +422,7 @@ template <int D, Part PART>
 struct Item {
     const mfft_cache& c;
     const mfft_attend_args& a;
-    const AttendShape& sh;
+    const ShapeOf<PART>& sh;
     Sequence seq;
     const int32_t* table;
     int h;
@@ -427,7 +430,7 @@ struct Item {
     int block_lo, block_hi, block_all_lo, block_all_hi;  // keys that any, and that all, rows of the block see
     bool all_see, some_blind;  // kPrefix: every row but blind ones sees all keys; there are blind ones
 
-    __device__ __forceinline__ Item(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_) : c(c_), a(a_), sh(sh_) {}
+    __device__ __forceinline__ Item(const mfft_cache& c_, const mfft_attend_args& a_, const ShapeOf<PART>& sh_) : c(c_), a(a_), sh(sh_) {}
 
     // the keys [lower, upper) that query `tok` of the sequence sees (kSinks: and
     // those of sink_keys)
@@ -485,7 +488,13 @@ struct Item {
         return {cut.parts, (slot + 1) * rows + (r & (rows - 1)), (slot + 2) * rows + (r & (rows - 1)), 2 * (int64_t)rows};
     }
     // kSinks: of rows that see [.., top) the keys [0, sink_keys(top)) too
-    __device__ __forceinline__ int sink_keys(int top) const { return PART == kSinks ? min(sh.sinks, top) : 0; }
+    __device__ __forceinline__ int sink_keys(int top) const {
+        if constexpr (PART == kSinks) return min(sh.sinks, top);
+        return 0;
+    }
+    // (not a comparison with 0 elsewhere: that a key's number is not negative the
+    // compiler does not know)
+    __device__ __forceinline__ bool in_sinks(int key, int top) const { return PART == kSinks && key < sink_keys(top); }
 
     // The keys of groups [tile, upto) of the item's list that rows of the block
     // see, as one run [from, end) of places.  The place of a key is its number;
@@ -648,7 +657,7 @@ struct Attend : Item<D, PART> {
     float cs, vs;
     int ve = 0;
 
-    __device__ __forceinline__ Attend(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
+    __device__ __forceinline__ Attend(const mfft_cache& c_, const mfft_attend_args& a_, const ShapeOf<PART>& sh_, Lds& lds_)
         : I(c_, a_, sh_), lds(lds_) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -777,7 +786,7 @@ struct Attend : Item<D, PART> {
     }
     __device__ __forceinline__ void take_scales(int key0) {
         const int kv = key0 + 16 * g;
-        vs = (kv + 16 > any_lo && kv < any_hi) || kv < this->sink_keys(any_hi) ? vs_raw : 1.0f;
+        vs = (kv + 16 > any_lo && kv < any_hi) || this->in_sinks(kv, any_hi) ? vs_raw : 1.0f;
         bool bad = bad_page;
         if constexpr (M::kShifts) {
             ve = M::shift(vs);
@@ -889,7 +898,7 @@ struct Attend : Item<D, PART> {
                 static_for<0, 4>([&](auto x) {
                     if ((vb[16 * (16 * i.value + x.value)] & 0x7f) == kNaNCode) {
                         static_for<0, R>([&](auto r) {
-                            if ((key >= low[r.value] && key < top[r.value]) || key < this->sink_keys(top[r.value]))
+                            if ((key >= low[r.value] && key < top[r.value]) || this->in_sinks(key, top[r.value]))
                                 o[r.value][i.value][x.value] = __builtin_nanf("");
                         });
                     }
@@ -1049,7 +1058,7 @@ struct Attend : Item<D, PART> {
                 entries(place + 128);
                 fetch(this->key_at(place + 64), e0);
             }
-            if ((key0 + 64 > any_lo && key0 < any_hi) || key0 < this->sink_keys(any_hi)) {
+            if ((key0 + 64 > any_lo && key0 < any_hi) || this->in_sinks(key0, any_hi)) {
                 f32x4 s[R][4];
                 x8 p[R][2];
                 const uint8_t* kb = lds.k[buf] + (16 * kg + kr) * KROW + 64 * kg;
@@ -1073,7 +1082,13 @@ struct Attend : Item<D, PART> {
 
     __device__ __forceinline__ void run(int tile, int upto) {
         int from, end;
-        this->span(tile, upto, from, end);
+        if constexpr (KEYS && PART == kAll) {
+            // the waves share the block's rows: what any of them sees is at hand
+            from = max(seq.low + 64 * tile, any_lo & ~63);
+            end = min(seq.low + 64 * upto, any_hi);
+        } else {
+            this->span(tile, upto, from, end);
+        }
         if constexpr (KEYS) run_keys(from, end);
         else run_rows(from, end);
         if constexpr (PART == kPrefix) clear_blind();
@@ -1158,7 +1173,7 @@ struct Tall : Item<D, PART> {
     bool large;  // some row's maximum has been past kFusedScores
     bool blind;  // see Attend
 
-    __device__ __forceinline__ Tall(const mfft_cache& c_, const mfft_attend_args& a_, const AttendShape& sh_, Lds& lds_)
+    __device__ __forceinline__ Tall(const mfft_cache& c_, const mfft_attend_args& a_, const ShapeOf<PART>& sh_, Lds& lds_)
         : I(c_, a_, sh_), lds(lds_) {
         lane = threadIdx.x & 63;
         wave = uniform((int)(threadIdx.x >> 6));
@@ -1254,7 +1269,7 @@ struct Tall : Item<D, PART> {
     }
     // whether some row of the block sees some of sixteen keys
     __device__ __forceinline__ bool block_sees(int kv) const {
-        return (kv + 16 > this->block_lo && kv < this->block_hi) || kv < this->sink_keys(this->block_hi);
+        return (kv + 16 > this->block_lo && kv < this->block_hi) || this->in_sinks(kv, this->block_hi);
     }
     __device__ __forceinline__ void stash(int buf, int key0) {
         const int kv = key0 + 16 * wave;
@@ -1410,7 +1425,7 @@ struct Tall : Item<D, PART> {
                 entries(place + 128);
                 fetch(this->key_at(place + 64), e0);
             }
-            if ((key0 + 64 > any_lo && key0 < any_hi) || key0 < this->sink_keys(any_hi)) {
+            if ((key0 + 64 > any_lo && key0 < any_hi) || this->in_sinks(key0, any_hi)) {
                 f32x16 s[2];
                 x8 p[4];
                 const uint8_t* kb = lds.k[buf] + k_at;
@@ -1458,7 +1473,7 @@ struct Tall : Item<D, PART> {
             if (!this->block_edge(key & ~63)) continue;
             const uint32_t u = (uint32_t)key >> 4;
             const uint8_t* vb = (const uint8_t*)c.v + this->unit_at(this->page_entry(u), u) + 64 * e + (key & 15);
-            const bool seen = (key >= low && key < top) || key < this->sink_keys(top);
+            const bool seen = (key >= low && key < top) || this->in_sinks(key, top);
             static_for<0, D / 32>([&](auto i) {
                 static_for<0, 16>([&](auto x) {
                     if ((vb[16 * (32 * i.value + 8 * (x.value / 4) + x.value % 4)] & 0x7f) == kNaNCode && seen)
@@ -1544,7 +1559,7 @@ __device__ __forceinline__ void clear_rest(const mfft_attend_args& a, int64_t i,
 }
 
 template <class E, int D, Form F, Part PART>
-__global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_cache c, mfft_attend_args a, AttendShape sh,
+__global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_cache c, mfft_attend_args a, ShapeOf<PART> sh,
                                                                           float* part_o, float2* part_ml, Cut* cuts) {
     using A = typename FormOf<E, D, F, PART>::type;
     __shared__ __align__(16) typename A::Lds lds;
@@ -1621,13 +1636,17 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
         w.run(tile, upto);
         if (tile == 0 && upto == w.seq.tiles) {
             w.store();
-            if (PART == kPrefix && sh.grid && threadIdx.x == 0 && number < sh.prefix.items) cuts[number].parts = 0;
+            if constexpr (PART == kPrefix) {
+                if (sh.grid && threadIdx.x == 0 && number < sh.prefix.items) cuts[number].parts = 0;
+            }
         } else {
             w.store_part(2 * (int)blockIdx.x + (tile == 0 ? 1 : 0), part_o, part_ml);
             if (tile == 0) {  // its last group lies `past` groups past this share's end
                 const int past = (int)(at + w.seq.tiles - 1 - stop);
                 cut = {share > past ? 2 : past / (int)share + 2, b, block, PART == kPrefix ? (int)blockIdx.x : h};
-                if (PART == kPrefix && threadIdx.x == 0 && number < sh.prefix.items) cuts[number] = cut;
+                if constexpr (PART == kPrefix) {
+                    if (threadIdx.x == 0 && number < sh.prefix.items) cuts[number] = cut;
+                }
             }
         }
         at += upto - tile;
@@ -1648,7 +1667,7 @@ __global__ __launch_bounds__(256, attend_per_cu(D, F)) void attend_kernel(mfft_c
 // many, all four waves every fourth part of one row after the other.  Each lane
 // takes D / 64 channels.
 template <class E, int D, Part PART>
-__global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_args a, AttendShape sh, const float* part_o,
+__global__ __launch_bounds__(256) void join_kernel(mfft_cache c, mfft_attend_args a, ShapeOf<PART> sh, const float* part_o,
                                                    const float2* part_ml, const Cut* cuts) {
     constexpr int C = (D + 63) / 64;
     const int groups = (sh.live + sh.join_rows - 1) / sh.join_rows;
