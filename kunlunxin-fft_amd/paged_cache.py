@@ -263,8 +263,9 @@ def append_paged_cache(cache: PagedCache, k, v, page_table, starts, *, offsets=N
 def read_paged_cache(cache: PagedCache, page_table, starts, tokens: int, *, offsets=None, dtype=torch.bfloat16):
     """The keys and values of cached tokens, two new tensors ``(tokens,
     kv_heads, head_dim)`` of ``dtype`` (float32, float16 or bfloat16): codes
-    times their page's scale, exact in float32 and bfloat16, rounded (and
-    infinite past its range) in float16.
+    times their page's scale, rounded once (infinite past the type's range).
+    Exact in float32 and bfloat16, but for codes of 256 and more under a scale
+    of 2^120, which are infinite, and, in bfloat16, for scales below 2^-124.
 
     The inverse of ``append_paged_cache``: rows ``offsets[b] .. offsets[b + 1]``
     (None: as many for every sequence) are sequence ``b``'s tokens from
