@@ -43,10 +43,11 @@
 // rows of one item, so that a code is fetched and decoded once for up to 128 of
 // them instead of once a sequence; it leaves m, l and O, unscaled, from which
 // each sequence's pass goes on: softmax is the same in any order of its keys.
-// 64 sequences of one token, 32768 shared keys and about 1000 of their own, 32
-// query and 8 key heads of 128: 89 us (without, 2.2 million keys are read
-// instead of 97 thousand), of which the shared keys' products, at 25 us by the
-// rate of a large matrix product, take 40.
+// 64 sequences of one token, 32768 shared keys and 1 to 1000 of their own, 32
+// query and 8 key heads of 128: 89 us (without, 2.1 million keys are read
+// instead of 65 thousand); in a trace the launch over the shared keys, whose
+// products are 25 us by the rate of a large matrix product, takes 62, the one over
+// the own keys, 66 MB, 31, and the join, which finds nothing cut, 5.
 #pragma once
 
 #include <algorithm>
@@ -184,9 +185,10 @@ __device__ __forceinline__ float moved_on(float m, float x, bool& large, S&& sco
 }
 
 // Whether a row that goes on from offset m may have scores past kFusedScores:
-// its largest lies at most 14 above m.
+// its largest lies at most kMost above m (float16's is the larger), and m is
+// rounded.
 __device__ __forceinline__ bool carried_large(float m) {
-    return __any(m > kLowest && __builtin_fabsf(m) > kFusedScores - 16.0f);
+    return __any(m > kLowest && __builtin_fabsf(m) > kFusedScores - (Mat<_Float16>::kMost + 1.0f));
 }
 
 // a mask of bytes [from, to) of a 16-byte unit
@@ -231,9 +233,9 @@ __device__ __forceinline__ float log_sum(float m, float l, bool poison) {
 // window of the first query on, also those that only later or earlier blocks of
 // rows see, which it leaves out.  Shares of a prompt piece over many cached
 // keys are so within a few percent of equal; those of a prompt of which nothing
-// is cached are not: 8192 tokens of 32 heads 1.16 ms, 475 TFLOP/s, where 2048
+// is cached are not: 8192 tokens of 32 heads 1.04 ms, 530 TFLOP/s, where 2048
 // over 32768 reach 910; nor those of a long piece in a short window: 2048
-// tokens in one of 512, 48 us.)  The list follows from the
+// tokens in one of 512, 43 us.)  The list follows from the
 // lengths, which only the device knows; every workgroup works its place out for
 // itself with one pass of a wave over the sequences.  Cut items leave their
 // (m, l, O) in the workspace and join_kernel adds them up.
