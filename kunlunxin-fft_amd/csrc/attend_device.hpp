@@ -1018,7 +1018,11 @@ struct Attend : Item<D, PART> {
             const int kv = key0 + 16 * wave;
             u32x4 keep = keep_bytes(this->block_lo - kv, this->block_hi - kv);
             if constexpr (PART == kSinks) keep |= keep_bytes(-kv, this->sink_keys(this->block_hi) - kv);
-            static_for<0, L>([&](auto x) { fv[x.value] = this->clean(fv[x.value], keep); });
+            static_for<0, L>([&](auto x) {
+                // (what a lane has not fetched may look like a NaN, and then all of the
+                // block's keys were looked through for it)
+                if (D % 64 == 0 || lane + 64 * x.value < D) fv[x.value] = this->clean(fv[x.value], keep);
+            });
             if (nan_left) lds.nan = 1;
         }
         static_for<0, L>([&](auto x) {
@@ -1278,7 +1282,9 @@ struct Tall : Item<D, PART> {
         if (this->block_edge(key0)) {
             u32x4 keep = keep_bytes(this->block_lo - kv, this->block_hi - kv);
             if constexpr (PART == kSinks) keep |= keep_bytes(-kv, this->sink_keys(this->block_hi) - kv);
-            static_for<0, L>([&](auto x) { fv[x.value] = this->clean(fv[x.value], keep); });
+            static_for<0, L>([&](auto x) {
+                if (D % 64 == 0 || lane + 64 * x.value < D) fv[x.value] = this->clean(fv[x.value], keep);  // see Attend
+            });
             if (nan_left) lds.nan = 1;
         }
         // keys that no row sees may have any scale, see Attend
