@@ -1371,11 +1371,17 @@ struct Tall : Item<D, PART> {
     // many products are made.  Left alone the compiler puts each load right before
     // its product, which then waits for it: 2048 tokens of 32 heads over 32768 took
     // 1241 us instead of 1179, the case of sinks above 189 instead of 178.  Eight
-    // ahead need more registers than two workgroups a CU have.
+    // ahead need more registers than two workgroups a CU have.  Head dim 64, with
+    // eight products where 128 has sixteen, is left to the compiler: 2048 tokens of
+    // 32 heads over 16384 406 us, 416 so, in float16 402 and 427.
     static constexpr int kAhead = 4;
     template <int N, class At, class Use>
     static __device__ __forceinline__ void products(At at, Use use) {
         static_assert(N % kAhead == 0);
+        if constexpr (D <= 64) {
+            static_for<0, N>([&](auto x) { use(x, *(const x8*)at(x)); });
+            return;
+        }
         x8 f[2][kAhead];
         static_for<0, kAhead>([&](auto x) { f[0][x.value] = *(const x8*)at(x); });
         static_for<0, N / kAhead>([&](auto b) {

@@ -34,7 +34,7 @@ AttendLaunch attend_launch(const mfft_cache& c, const mfft_attend_args& a, const
     //   dim 64   kKeys1 33 35 36 71 59 82 86, kKeys2 39 40 39 46 46 76 79, kKeys4 55 54 53 53 55 97 97,
     //            kRows 68 67 66 66 66 97 96, kTall 90 89 87 88 87 88 90
     //   dim 96   kKeys1 43 40 41 100 71 103 117, kKeys2 48 49 49 52 52 107 95, kKeys4 59 60 60 61 63 110 110,
-    //            kRows 77 78 78 78 79 330 328, kTall 114 116 116 117 117 120 124
+    //            kRows 77 78 78 78 79 113 113, kTall 114 116 116 117 117 120 124
     //   dim 128  kKeys1 55 56 57 133 99 137 168, kKeys2 51 51 52 93 94 133 156, kKeys4 75 76 77 78 80 140 143,
     //            kRows 86 88 86 90 91 138 138, kTall 117 119 117 121 121 125 130
     //   dim 256  kKeys1 57 91 92 130 165 242 194, kRows 89 91 91 93 96 143 143
